@@ -26,8 +26,9 @@ CSRC = PKG_DIR / "csrc"
 BUILD_DIR = PKG_DIR / "_build"
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 
-CU_SOURCES = ["ppb_common.cu", "pool_kernels.cu", "engine.cu", "native_ops.cu", "noalloc.cu", "vmm.cu"]
-CC_SOURCES = ["planner.cc", "host_ops.cc", "bindings.cc", "bind_ops.cc"]
+CU_SOURCES = ["ppb_common.cu", "pool_kernels.cu", "engine.cu", "native_ops.cu", "noalloc.cu", "vmm.cu",
+              "kv_attention.cu", "kv_blocks.cu"]
+CC_SOURCES = ["planner.cc", "host_ops.cc", "bindings.cc", "bind_ops.cc", "bind_kv.cc"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

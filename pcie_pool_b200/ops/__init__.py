@@ -10,6 +10,7 @@ from __future__ import annotations
 import numpy as np
 
 from .._native import native
+from .paged_kv import KVEviction, paged_kv_attention, paged_kv_bounds, paged_kv_evict, paged_kv_select
 
 
 def _torch():
