@@ -49,7 +49,7 @@ void bind_kv(py::module_& m) {
       .def("work_bytes",
            [](const KvAttention& a, int device) {
              DeviceGuard guard(device);
-             return paged_kv_attention_work(a, device);
+             return paged_kv_attention_work(a);
            })
       .def("run", [](KvAttention a, uint64_t out, uint64_t lse, uint64_t work, int device, uint64_t stream) {
         DeviceGuard guard(device);

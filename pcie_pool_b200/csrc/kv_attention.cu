@@ -2,129 +2,620 @@
 //
 //   s_t = scale * <q, K_t>,  out = sum_t exp(s_t - lse) V_t,  lse = log sum_t exp(s_t)
 //   mass_j += sum over heads and the tokens t of block j of exp(s_t - lse)
+//
+// Every key and value is read once and used for the G query heads of its key
+// head: 2 G flops a byte, so the cache's bytes bound it, not the arithmetic.  A
+// warp works alone: it streams tiles of 16 tokens of one key head through its
+// own ring of shared memory (cp.async, 16 bytes a lane, a page looked up one
+// tile ahead) and keeps the G x dim result in registers with the running maximum
+// and sum of the softmax.  No barrier stands in the loop, and tiles of the next
+// request are already on their way while the last one is finished.  Consecutive
+// warps take the key heads of the same tokens, so a page's rows, which lie next
+// to each other, are fetched together.  kv_plan.h says how the tiles are shared
+// out and attention_join_kernel adds up what was cut.
+//
+// The products run on mma.m16n8k16 with the heads as rows: a token's 16 columns
+// cost the same whether 1 or 16 heads use them, and at 16 tokens a step the tensor
+// pipe is far from its limit (tcgen05's 128 rows would be 4 or 8 heads and
+// padding).  Weights are multiplied as two numbers of the cache's type, high part and
+// remainder, so the result is as exact as with weights in fp32; up to eight
+// heads, the remainders are the eight rows that the heads leave free and cost nothing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <cmath>
 
+#include "device_utils.cuh"
+#include "kv_plan.h"
 #include "paged_kv.h"
 
 namespace ppb {
 namespace {
 
-constexpr int kTile = 16;  // tokens of a step; the mass is gathered by tiles
+constexpr int kTile = 16;      // tokens of a step; the mass is gathered by tiles
+constexpr int kLeastTiles = 2; // of a range: shorter ones cost more to join than they save
+constexpr int kRowGroup = 16;  // query heads of one warp at most
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_f(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f(__half& o, float v) { o = __float2half_rn(v); }
+// Warps of a CTA and tiles in flight of each, by the padded dim: about 192 KiB
+// of shared memory, one CTA to an SM.
+template <int DP>
+struct Shape {
+  static constexpr int kWarps = DP == 256 ? 4 : 8;
+  static constexpr int kStages = DP == 64 ? 6 : 3;
+  static constexpr int kStageBytes = 2 * kTile * DP * 2;  // K, then V
+  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+};
 
-// Blocks of request b that are read: all that hold tokens, or the listed ones.
+struct Work {
+  float* part_o;        // [2 ranges, groups, rows, dim]
+  float2* part_ml;      // [2 ranges, groups, rows]: maximum (base 2) and sum
+  uint32_t* first;      // [requests + 1]
+  float* z;             // [requests, max_tiles, heads]: log2 of a tile's sum, or null
+  int max_tiles;        // of a request
+  int most_ranges;
+  int groups;           // kv_heads * row groups
+  int rows;             // of a group's partial result: 8 or 16
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_parent() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename T>
+struct Type;
+
+template <>
+struct Type<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<uint32_t&>(v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+};
+
+template <>
+struct Type<__half> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return reinterpret_cast<uint32_t&>(v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return __half22float2(reinterpret_cast<__half2&>(v));
+  }
+};
+
+// High part of two weights and what it leaves, as pairs.
+template <typename T>
+__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = Type<T>::pack(x, y);
+  const float2 h = Type<T>::unpack(hi);
+  lo = Type<T>::pack(x - h.x, y - h.y);
+}
+
+__device__ __forceinline__ int length_of(const KvAttention& a, int b) {
+  const long long most = static_cast<long long>(a.req.width) * a.kv.block;
+  return max(0, static_cast<int>(min(static_cast<long long>(a.req.lens[b]), most)));
+}
+
+// Blocks of a request that are read: all that hold tokens, or the listed ones.
 __device__ __forceinline__ int slots_of(const KvAttention& a, int len) {
   const int n = (len + a.kv.block - 1) / a.kv.block;
   return a.blocks != nullptr && a.blocks_width < n ? a.blocks_width : n;
 }
 
-// One CTA for each query head of a request, four warps that take tiles in turn.
-template <typename T>
-__global__ void __launch_bounds__(128) attention_kernel(KvAttention a, float* __restrict__ z, int max_tiles) {
-  const int b = blockIdx.y, h = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int D = a.kv.dim, g = h / (a.heads / a.kv.kv_heads);
-  const long long most = (long long)a.req.width * a.kv.block;
-  const int len = max(0, (int)min((long long)a.req.lens[b], most));
-  const int slots = slots_of(a, len), tiles = (int)(((long long)slots * a.kv.block + kTile - 1) / kTile);
-  const T* qp = (const T*)a.q + b * a.q_stride + h * a.q_head_stride;
-  const T* kp = (const T*)a.kv.base + g * a.kv.head_stride;
-  float q[8], o[8], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < 8; ++i) {
-    q[i] = lane + 32 * i < D ? to_f(qp[lane + 32 * i]) : 0.f;
-    o[i] = 0.f;
-  }
-  for (int tile = warp; tile < tiles; tile += 4) {
-    float zm = -INFINITY, zl = 0.f;
-    for (int r = 0; r < kTile; ++r) {
-      const long long t = (long long)tile * kTile + r;
-      const int slot = (int)(t / a.kv.block), off = (int)(t % a.kv.block);
-      if (slot >= slots) break;
-      const int lb = a.blocks ? a.blocks[((long long)b * a.kv.kv_heads + g) * a.blocks_width + slot] : slot;
-      if (lb < 0 || (long long)lb * a.kv.block + off >= len) continue;
-      const int page = a.req.table[b * a.req.table_stride + lb];
-      if (page < 0 || page >= a.kv.pages) continue;
-      const T* k = kp + page * a.kv.page_stride + off * a.kv.token_stride;
-      float s = 0.f;
-      for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < D) s += q[i] * to_f(k[lane + 32 * i]);
-      for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= a.scale;
-      if (s == -INFINITY) continue;
-      const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.f : expf(m - mn), p = expf(s - mn);
-      m = mn;
-      l = l * c + p;
-      for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < D) o[i] = o[i] * c + p * to_f(k[a.kv.lane_stride + lane + 32 * i]);
-      const float zn = fmaxf(zm, s);
-      zl = (zm == -INFINITY ? 0.f : zl * expf(zm - zn)) + expf(s - zn);
-      zm = zn;
-    }
-    if (z && lane == 0) z[((long long)b * max_tiles + tile) * a.heads + h] = zm + logf(zl);
-  }
-  __shared__ float sm[4], sl[4], so[4][256];
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < D) so[warp][lane + 32 * i] = o[i];
-  __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float w[4], total = 0.f;
-  for (int i = 0; i < 4; ++i) {
-    w[i] = sm[i] == -INFINITY ? 0.f : expf(sm[i] - top);
-    total += w[i] * sl[i];
-  }
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float v = 0.f;
-    for (int i = 0; i < 4; ++i) v += w[i] * so[i][d];
-    from_f(((T*)a.out)[((long long)b * a.heads + h) * D + d], total == 0.f ? 0.f : v / total);
-  }
-  if (threadIdx.x == 0) a.lse[(long long)b * a.heads + h] = total == 0.f ? -INFINITY : top + logf(total);
+__device__ __forceinline__ uint32_t tiles_of(const KvAttention& a, int len) {
+  return static_cast<uint32_t>((static_cast<long long>(slots_of(a, len)) * a.kv.block + kTile - 1) / kTile);
 }
 
-// A warp for each block: the tiles' log-sums of every head, weighed by the head's total.
-__global__ void __launch_bounds__(128) mass_kernel(KvAttention a, const float* __restrict__ z, int max_tiles) {
-  const int b = blockIdx.y, j = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const long long most = (long long)a.req.width * a.kv.block;
-  const int len = max(0, (int)min((long long)a.req.lens[b], most));
-  if (j >= (len + a.kv.block - 1) / a.kv.block) return;
-  const int per = a.kv.block / kTile, last = (len + kTile - 1) / kTile;
-  float sum = 0.f;
-  for (int t = j * per; t < min((j + 1) * per, last); ++t)
-    for (int h = lane; h < a.heads; h += 32) {
-      const float v = z[((long long)b * max_tiles + t) * a.heads + h];
-      if (v != -INFINITY) sum += expf(v - a.lse[(long long)b * a.heads + h]);
+// first[b] of every request and of their end, by the whole CTA.
+__device__ __forceinline__ void first_tiles(const KvAttention& a, uint32_t* first, uint32_t* scratch) {
+  const int n = a.req.requests, per = (n + blockDim.x - 1) / blockDim.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int b0 = min(n, static_cast<int>(threadIdx.x) * per), b1 = min(n, b0 + per);
+  uint32_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    first[b] = mine;
+    mine += tiles_of(a, length_of(a, b));
+  }
+  uint32_t upto = mine;
+#pragma unroll
+  for (int x = 1; x < 32; x *= 2) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, x);
+    if (lane >= x) upto += v;
+  }
+  if (lane == 31) scratch[warp] = upto;
+  __syncthreads();
+  uint32_t before = upto - mine;
+  for (int w = 0; w < warp; ++w) before += scratch[w];
+  for (int b = b0; b < b1; ++b) first[b] += before;
+  if (threadIdx.x == blockDim.x - 1) first[n] = before + mine;
+  __syncthreads();
+}
+
+// The request of a tile: the last b with first[b] <= tile that has tiles.
+__device__ __forceinline__ int request_of(const uint32_t* first, int n, uint32_t tile) {
+  int lo = 0, hi = n;  // first[lo] <= tile < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] <= tile)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// DP: dim padded to 64, 128 or 256.  PACKED: at most eight heads share a key head,
+// rows 8 to 15 carry the weights' remainders.
+template <typename T, int DP, bool PACKED>
+__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
+    attention_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w) {
+  using S = Shape<DP>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t scratch[S::kWarps];
+  __shared__ uint32_t valid_of[S::kWarps][S::kStages];
+  uint32_t* first = reinterpret_cast<uint32_t*>(smem + S::kRingBytes);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int D = a.kv.dim, bs = a.kv.block, G = a.heads / a.kv.kv_heads, n = a.req.requests;
+  launch_dependents();
+  if (D < DP)  // what the copies leave of a row stays zero
+    for (int i = threadIdx.x; i < S::kRingBytes / 16; i += blockDim.x)
+      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  first_tiles(a, first, scratch);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= n; i += blockDim.x) w.first[i] = first[i];
+  const KvPlan plan = KvPlan::make(first[n], w.most_ranges, kLeastTiles);
+  if (plan.tiles == 0) return;
+  const long long units = static_cast<long long>(plan.ranges) * w.groups;
+  // few units: one to a CTA before two
+  const int per_cta = static_cast<int>(min(static_cast<long long>(S::kWarps), (units + gridDim.x - 1) / gridDim.x));
+  if (warp >= per_cta) return;
+  const uint32_t ring = dev::smem_u32(smem) + warp * S::kStages * S::kStageBytes;
+
+  for (long long unit = static_cast<long long>(blockIdx.x) * per_cta + warp; unit < units;
+       unit += static_cast<long long>(gridDim.x) * per_cta) {
+    const int r = static_cast<int>(unit / w.groups), group = static_cast<int>(unit % w.groups);
+    const int per_head = (G + kRowGroup - 1) / kRowGroup, g = group / per_head, row0 = group % per_head * kRowGroup;
+    const int rows = min(kRowGroup, G - row0);
+    const uint32_t lo = static_cast<uint32_t>(plan.begin(r)), hi = static_cast<uint32_t>(plan.begin(r + 1));
+    const T* cache = static_cast<const T*>(a.kv.base) + g * a.kv.head_stride;
+
+    // ---- the tiles' places and copies --------------------------------------------
+    uint32_t next = lo;  // the tile that is looked up next
+    int lb = request_of(first, n, lo), llen = length_of(a, lb), lslots = slots_of(a, llen);
+    long long row_at = 0;  // of lanes 0-15: where the row of the tile looked up last begins
+    bool row_ok = false;
+    auto look_up = [&]() {
+      row_ok = false;
+      if (next < hi) {
+        while (next >= first[lb + 1]) {
+          ++lb;
+          llen = length_of(a, lb);
+          lslots = slots_of(a, llen);
+        }
+        const uint32_t t = (next - first[lb]) * kTile + (lane & 15);
+        const int slot = static_cast<int>(t / static_cast<uint32_t>(bs)), off = static_cast<int>(t - slot * static_cast<uint32_t>(bs));
+        int block = slot;
+        bool ok = slot < lslots;
+        if (a.blocks != nullptr) {
+          block = ok ? a.blocks[(static_cast<long long>(lb) * a.kv.kv_heads + g) * a.blocks_width + slot] : -1;
+          ok = block >= 0;
+        }
+        ok = ok && static_cast<long long>(block) * bs + off < llen;
+        const int page = ok ? a.req.table[lb * a.req.table_stride + block] : -1;
+        row_ok = page >= 0 && page < a.kv.pages;
+        row_at = row_ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
+      }
+      ++next;
+    };
+    constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
+    auto copy = [&](int stage) {
+      const uint32_t ok = __ballot_sync(0xffffffffu, row_ok) & 0xffffu;
+      if (lane == 0) valid_of[warp][stage] = ok;
+      const uint32_t to = ring + stage * S::kStageBytes;
+#pragma unroll
+      for (int i = 0; i < kTile * kChunks / 32; ++i) {
+        const int row = (i * 32 + lane) / kChunks, chunk = (i * 32 + lane) % kChunks;
+        const long long at = __shfl_sync(0xffffffffu, row_at, row) + chunk * 8;
+        const uint32_t dst = to + row * DP * 2 + ((chunk ^ (row & 7)) * 16);
+        if (chunk * 8 < D) {
+          const T* src = cache + at;
+          const bool v = ok >> row & 1;
+          cp_async16(dst, v ? src : a.kv.base, v);
+          cp_async16(dst + kTile * DP * 2, v ? src + a.kv.lane_stride : a.kv.base, v);
+        }
+      }
+    };
+    look_up();
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+      if (lo + i < hi) copy(i);
+      cp_commit();
+      look_up();
     }
-  for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+
+    // ---- the products ----------------------------------------------------------------
+    float o[DP / 8][4], m[2], l[2];
+    uint32_t q[DP / 16][4];
+    const float to_base2 = a.scale * kLog2e;
+    int b = -1;
+    uint32_t end = 0;  // of request b's tiles
+    int stage = 0;
+    for (uint32_t tile = lo; tile < hi; ++tile) {
+      if (b < 0 || tile >= end) {  // a new request: its heads' rows
+        b = b < 0 ? request_of(first, n, tile) : b + 1;
+        while (first[b + 1] <= tile) ++b;
+        end = first[b + 1];
+        const T* qp = static_cast<const T*>(a.q) + b * a.q_stride + (g * G + row0) * a.q_head_stride;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+            q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
+                          ? 0u
+                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q_head_stride + d);
+          }
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+      }
+      cp_wait<S::kStages - 2>();
+      __syncwarp();
+      {  // the stage that the last step emptied
+        const int into = stage == 0 ? S::kStages - 1 : stage - 1;
+        if (tile + S::kStages - 1 < hi) copy(into);
+        cp_commit();
+        look_up();
+      }
+      const uint32_t ok = valid_of[warp][stage];
+      const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + kTile * DP * 2;
+      float s[2][4] = {};
+      {
+        const int row = (lane & 7) + ((lane >> 4) << 3);
+        const uint32_t base = ks + row * DP * 2;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          uint32_t f[4];
+          ldsm4(f, base + (((2 * k + ((lane >> 3) & 1)) ^ (row & 7)) * 16));
+          Type<T>::mma(s[0], q[k], f[0], f[1]);
+          Type<T>::mma(s[1], q[k], f[2], f[3]);
+        }
+      }
+      constexpr int kHalves = PACKED ? 1 : 2;  // row lane / 4, and the one eight below
+      bool grew = false;
+      float ratio[2];
+#pragma unroll
+      for (int x = 0; x < kHalves; ++x) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = (lane & 3) * 2 + (i & 1) + (i >> 1) * 8;
+          float& v = s[i >> 1][2 * x + (i & 1)];
+          v = ok >> col & 1 ? v * to_base2 : -INFINITY;
+          top = fmaxf(top, v);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float now = fmaxf(m[x], top), at = now == -INFINITY ? 0.f : now;
+        ratio[x] = ex2(m[x] - at);
+        grew |= now > m[x];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float& v = s[i >> 1][2 * x + (i & 1)];
+          v = ex2(v - at);
+          sum += v;
+        }
+        m[x] = now;
+        l[x] = l[x] * ratio[x] + sum;  // of this lane's columns
+        if (w.z != nullptr) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          const int row = lane / 4 + 8 * x;
+          if ((lane & 3) == 0 && row < rows)
+            w.z[(static_cast<long long>(b) * w.max_tiles + (tile - first[b])) * a.heads + g * G + row0 + row] = at + lg2(sum);
+        }
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+          o[i][0] *= ratio[0];
+          o[i][1] *= ratio[0];
+          o[i][2] *= ratio[kHalves - 1];
+          o[i][3] *= ratio[kHalves - 1];
+        }
+      }
+      uint32_t p[4], rest[4];
+      if constexpr (PACKED) {
+        split<T>(s[0][0], s[0][1], p[0], p[1]);
+        split<T>(s[1][0], s[1][1], p[2], p[3]);
+      } else {
+        split<T>(s[0][0], s[0][1], p[0], rest[0]);
+        split<T>(s[0][2], s[0][3], p[1], rest[1]);
+        split<T>(s[1][0], s[1][1], p[2], rest[2]);
+        split<T>(s[1][2], s[1][3], p[3], rest[3]);
+      }
+      {
+        const int row = lane & 15;
+        const uint32_t base = vs + row * DP * 2;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          uint32_t f[4];
+          ldsm4_t(f, base + (((2 * k + (lane >> 4)) ^ (row & 7)) * 16));
+          Type<T>::mma(o[2 * k], p, f[0], f[1]);
+          Type<T>::mma(o[2 * k + 1], p, f[2], f[3]);
+          if constexpr (!PACKED) {
+            Type<T>::mma(o[2 * k], rest, f[0], f[1]);
+            Type<T>::mma(o[2 * k + 1], rest, f[2], f[3]);
+          }
+        }
+      }
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+
+      if (tile + 1 == end || tile + 1 == hi) {  // the request's or the range's last
+        const bool whole = first[b] >= lo && end <= hi;
+        const int slot = plan.slot(r, first[b]);
+#pragma unroll
+        for (int x = 0; x < kHalves; ++x) {
+          const int row = lane / 4 + 8 * x;
+          float sum = l[x];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          if (row >= rows) continue;
+          const int h = g * G + row0 + row;
+          const long long at = static_cast<long long>(slot) * w.groups * w.rows + static_cast<long long>(group) * w.rows + row;
+          const float by = sum == 0.f ? 0.f : 1.f / sum;
+          if ((lane & 3) == 0) {
+            if (whole)
+              a.lse[static_cast<long long>(b) * a.heads + h] = sum == 0.f ? -INFINITY : (m[x] + lg2(sum)) * kLn2;
+            else
+              w.part_ml[at] = make_float2(m[x], sum);
+          }
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            const int d = i * 8 + (lane & 3) * 2;
+            const float u = PACKED ? o[i][0] + o[i][2] : o[i][2 * x], v = PACKED ? o[i][1] + o[i][3] : o[i][2 * x + 1];
+            if (d < D) {
+              if (whole)
+                *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (static_cast<long long>(b) * a.heads + h) * D + d) =
+                    Type<T>::pack(sum == 0.f ? 0.f : u * by, sum == 0.f ? 0.f : v * by);
+              else
+                *reinterpret_cast<float2*>(w.part_o + at * D + d) = make_float2(u, v);
+            }
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncwarp();
+  }
+}
+
+// Adds up what the ranges left of a request that was cut: a CTA for each query
+// head, its warps take the parts in turn.  Requests without tokens get zeros.
+constexpr int kJoinWarps = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ KvAttention a,
+                                                                         const __grid_constant__ Work w) {
+  __shared__ float sum_o[kJoinWarps][256], sum_m[kJoinWarps], sum_l[kJoinWarps];
+  const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int D = a.kv.dim;
+  wait_for_parent();
+  const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
+  T* out = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.heads + h) * D;
+  float* lse = a.lse + static_cast<long long>(b) * a.heads + h;
+  if (f0 == f1) {
+    for (int d = 2 * threadIdx.x; d < D; d += 2 * blockDim.x) *reinterpret_cast<uint32_t*>(out + d) = 0u;
+    if (threadIdx.x == 0) *lse = -INFINITY;
+    return;
+  }
+  const KvPlan plan = KvPlan::make(w.first[a.req.requests], w.most_ranges, kLeastTiles);
+  const int r0 = plan.of(f0), r1 = plan.of(f1 - 1);
+  if (r0 == r1) return;  // finished where it was computed
+  const int G = a.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
+  const int group = h / G * per_head + h % G / kRowGroup, row = h % G % kRowGroup;
+  float m = -INFINITY, l = 0.f, o[8] = {};
+  for (int r = r0 + warp; r <= r1; r += kJoinWarps) {
+    const long long at = (static_cast<long long>(plan.slot(r, f0)) * w.groups + group) * w.rows + row;
+    const float2 ml = w.part_ml[at];
+    float4 v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i * 128 + lane * 4 < D) v[i] = *reinterpret_cast<const float4*>(w.part_o + at * D + i * 128 + lane * 4);
+    const float now = fmaxf(m, ml.x), ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref), p = ex2(ml.x - ref);
+    m = now;
+    l = l * c + ml.y * p;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i * 128 + lane * 4 < D) {
+        o[4 * i] = o[4 * i] * c + v[i].x * p;
+        o[4 * i + 1] = o[4 * i + 1] * c + v[i].y * p;
+        o[4 * i + 2] = o[4 * i + 2] * c + v[i].z * p;
+        o[4 * i + 3] = o[4 * i + 3] * c + v[i].w * p;
+      }
+  }
+  if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = i / 4 * 128 + lane * 4 + i % 4;
+    if (d < D) sum_o[warp][d] = o[i];
+  }
+  __syncthreads();
+  float top = -INFINITY, total = 0.f, by[kJoinWarps];
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, sum_m[i]);
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) {
+    by[i] = ex2(sum_m[i] - (top == -INFINITY ? 0.f : top));
+    total += by[i] * sum_l[i];
+  }
+  for (int d = 2 * threadIdx.x; d < D; d += 2 * blockDim.x) {
+    float u = 0.f, v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) {
+      u += by[i] * sum_o[i][d];
+      v += by[i] * sum_o[i][d + 1];
+    }
+    *reinterpret_cast<uint32_t*>(out + d) = total == 0.f ? 0u : Type<T>::pack(u / total, v / total);
+  }
+  if (threadIdx.x == 0) *lse = total == 0.f ? -INFINITY : (top + lg2(total)) * kLn2;
+}
+
+// A warp for each block: the tiles' sums of every head, weighed by the head's total.
+__global__ void __launch_bounds__(128) mass_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w) {
+  const int b = blockIdx.y, j = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  wait_for_parent();
+  const int len = length_of(a, b);
+  if (j >= (len + a.kv.block - 1) / a.kv.block) return;
+  const int per = a.kv.block / kTile, t0 = j * per, t1 = min(t0 + per, (len + kTile - 1) / kTile);
+  float sum = 0.f;
+  for (int h = lane; h < a.heads; h += 32) {
+    const float total = a.lse[static_cast<long long>(b) * a.heads + h] * kLog2e;
+    for (int t = t0; t < t1; ++t) {
+      const float v = w.z[(static_cast<long long>(b) * w.max_tiles + t) * a.heads + h];
+      sum += v == -INFINITY ? 0.f : ex2(v - total);
+    }
+  }
+  sum = dev::warp_sum(sum);
   if (lane == 0) a.mass[b * a.mass_stride + j] += sum;
 }
 
-int max_tiles(const KvAttention& a) {
-  return static_cast<int>(((long long)a.req.width * a.kv.block + kTile - 1) / kTile);
+int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
+
+// The workspace's parts behind `base`; returns its size.
+uint64_t lay_out(const KvAttention& a, int sms, void* base, Work& w) {
+  const int G = a.heads / a.kv.kv_heads, warps = sms * (padded(a.kv.dim) == 256 ? Shape<256>::kWarps : Shape<128>::kWarps);
+  w.groups = a.kv.kv_heads * ((G + kRowGroup - 1) / kRowGroup);
+  w.rows = G <= 8 ? 8 : 16;
+  w.most_ranges = warps / w.groups > 0 ? warps / w.groups : 1;
+  w.max_tiles = static_cast<int>((static_cast<int64_t>(a.req.width) * a.kv.block + kTile - 1) / kTile);
+  const uint64_t parts = 2ull * w.most_ranges * w.groups * w.rows;
+  uint8_t* p = static_cast<uint8_t*>(base);
+  uint64_t at = 0;
+  w.part_o = reinterpret_cast<float*>(p + at);
+  at += up(parts * a.kv.dim * 4);
+  w.part_ml = reinterpret_cast<float2*>(p + at);
+  at += up(parts * 8);
+  w.first = reinterpret_cast<uint32_t*>(p + at);
+  at += up((a.req.requests + 1ull) * 4);
+  w.z = a.mass ? reinterpret_cast<float*>(p + at) : nullptr;
+  if (a.mass) at += up(uint64_t(a.req.requests) * w.max_tiles * a.heads * 4);
+  return at;
+}
+
+cudaError_t sm_count(int* sms) {
+  int device = 0;
+  cudaError_t rc = cudaGetDevice(&device);
+  return rc != cudaSuccess ? rc : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+}
+
+// A kernel that may be resident before the one ahead of it in the stream is done
+// (it waits for it itself).
+template <typename... Args>
+cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t stream, const KvAttention& a,
+                         const Work& w) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, a, w);
+}
+
+template <typename T, int DP>
+cudaError_t launch(const KvAttention& a, const Work& w, int sms, cudaStream_t stream) {
+  const int smem = Shape<DP>::kRingBytes + (a.req.requests + 1) * 4, threads = Shape<DP>::kWarps * 32;
+  auto kernel = w.rows == 8 ? attention_kernel<T, DP, true> : attention_kernel<T, DP, false>;
+  cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (rc != cudaSuccess) return rc;
+  kernel<<<sms, threads, smem, stream>>>(a, w);
+  rc = cudaGetLastError();
+  if (rc != cudaSuccess) return rc;
+  return launch_after(attention_join_kernel<T>, dim3(a.req.requests * a.heads), kJoinWarps * 32, stream, a, w);
+}
+
+template <typename T>
+cudaError_t launch(const KvAttention& a, const Work& w, int sms, cudaStream_t stream) {
+  switch (padded(a.kv.dim)) {
+    case 64: return launch<T, 64>(a, w, sms, stream);
+    case 128: return launch<T, 128>(a, w, sms, stream);
+    default: return launch<T, 256>(a, w, sms, stream);
+  }
 }
 
 }  // namespace
 
-uint64_t paged_kv_attention_work(const KvAttention& a, int) {
-  return a.mass ? uint64_t(a.req.requests) * max_tiles(a) * a.heads * 4 : 0;
+uint64_t paged_kv_attention_work(const KvAttention& a) {
+  int sms = 0;
+  Work w;
+  return sm_count(&sms) == cudaSuccess ? lay_out(a, sms, nullptr, w) : 0;
 }
 
 cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream) {
   if (a.req.requests == 0) return cudaSuccess;
-  float* z = a.mass ? static_cast<float*>(a.work) : nullptr;
-  const dim3 grid(a.heads, a.req.requests);
-  if (a.kv.type == kKvBf16)
-    attention_kernel<__nv_bfloat16><<<grid, 128, 0, stream>>>(a, z, max_tiles(a));
-  else
-    attention_kernel<__half><<<grid, 128, 0, stream>>>(a, z, max_tiles(a));
-  if (a.mass && a.req.width)
-    mass_kernel<<<dim3((a.req.width + 3) / 4, a.req.requests), 128, 0, stream>>>(a, z, max_tiles(a));
-  return cudaGetLastError();
+  int sms = 0;
+  cudaError_t rc = sm_count(&sms);
+  if (rc != cudaSuccess) return rc;
+  Work w;
+  lay_out(a, sms, a.work, w);
+  rc = a.kv.type == kKvBf16 ? launch<__nv_bfloat16>(a, w, sms, stream) : launch<__half>(a, w, sms, stream);
+  if (rc == cudaSuccess && a.mass && a.req.width)
+    rc = launch_after(mass_kernel, dim3((a.req.width + 3) / 4, a.req.requests), 128, stream, a, w);
+  return rc;
 }
 
 }  // namespace ppb

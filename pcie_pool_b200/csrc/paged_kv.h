@@ -48,8 +48,8 @@ struct KvAttention {
   void* work = nullptr;    // paged_kv_attention_work() bytes
 };
 
-// Workspace bytes of a call (its pointers are not read).
-uint64_t paged_kv_attention_work(const KvAttention& a, int device);
+// Workspace bytes of a call on the current device (its pointers are not followed).
+uint64_t paged_kv_attention_work(const KvAttention& a);
 cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream);
 
 // Bounds [pages, kv_heads, 2, dim] (smallest, then largest key of each channel) of

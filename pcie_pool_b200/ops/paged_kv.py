@@ -36,6 +36,7 @@ from .._native import native
 
 MAX_REQUESTS = 8192
 MAX_DIM = 256
+MAX_BLOCK = 65536
 
 
 def _torch():
@@ -81,7 +82,9 @@ def _requests(block_table, context_lens, device, block: int):
           "context_lens must be int32 [requests]")
     _need(block_table.device == device and context_lens.device == device, "all tensors must be on one CUDA device")
     _need(n <= MAX_REQUESTS, f"at most {MAX_REQUESTS} requests")
-    _need(width * block < 2**31 - 64, "block_table is too wide: a request has at most 2**31 tokens")
+    _need(block <= MAX_BLOCK, f"at most {MAX_BLOCK} tokens a block")
+    _need(width * block <= 2**31 - 2 * MAX_BLOCK, "block_table is too wide: a request has at most 2**31 tokens")
+    _need(n * width * block < 2**35, "block_table is too large: at most 2**35 tokens in all")
     _need(width <= 1 or block_table.stride(1) == 1, "block_table's rows must be contiguous")
     _need(n <= 1 or context_lens.stride(0) == 1, "context_lens must be contiguous")
     return native().KvRequests(block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), n, width)
@@ -110,7 +113,7 @@ def _query(q, device, dtype, dim: int, kv_heads: int, requests: int):
           "q's dim must be the cache's, and its heads a multiple of the cache's")
     # pairs are loaded at once: a view that splits them is copied
     if q.stride(2) != 1 or (q.data_ptr() | 2 * q.stride(0) | 2 * q.stride(1)) % 4:
-        q = q.contiguous()
+        q = q.clone(memory_format=_torch().contiguous_format)
     return q
 
 
@@ -166,8 +169,8 @@ def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=N
         _need((width <= 1 or mass.stride(1) == 1) and (n <= 1 or mass.stride(0) >= width),
               "mass must have contiguous rows of their own")
     if out is not None:
-        _need(out.dtype == q.dtype and out.device == dev and out.shape == q.shape and out.is_contiguous(),
-              "out must be contiguous and like q")
+        _need(out.dtype == q.dtype and out.device == dev and out.shape == q.shape and out.is_contiguous()
+              and out.data_ptr() % 4 == 0, "out must be contiguous, like q, on a 4-byte boundary")
         _need(not _overlap(out, q) and not _overlap(out, kv), "out must not overlap q or kv")
     _cuda(dev)
     if out is None:

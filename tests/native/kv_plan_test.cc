@@ -1,0 +1,67 @@
+// The attention kernel's cut of its work (csrc/kv_plan.h): every tile in one
+// range, every partial result in a place of its own within the workspace, and
+// the join looks in exactly the places that were written.
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <set>
+#include <vector>
+
+#include "kv_plan.h"
+
+using ppb::KvPlan;
+
+#define CHECK(x)                                                     \
+  do {                                                               \
+    if (!(x)) {                                                      \
+      std::printf("failed at line %d: %s\n", __LINE__, #x);          \
+      std::exit(1);                                                  \
+    }                                                                \
+  } while (0)
+
+static void check(const std::vector<int64_t>& tiles, int most, int least) {
+  std::vector<int64_t> first{0};
+  for (int64_t t : tiles) first.push_back(first.back() + t);
+  const KvPlan p = KvPlan::make(first.back(), most, least);
+  CHECK(p.ranges >= 1 && p.ranges <= most);
+  if (p.tiles == 0) return;
+  CHECK(p.begin(0) == 0 && p.begin(p.ranges) == p.tiles);
+  std::set<std::pair<size_t, int>> written;  // (request, slot)
+  std::set<int> slots;
+  size_t b = 0;
+  for (int r = 0; r < p.ranges; ++r) {
+    const int64_t lo = p.begin(r), hi = p.begin(r + 1);
+    CHECK(lo < hi);  // ranges are never more than tiles
+    CHECK(p.of(lo) == r && p.of(hi - 1) == r);
+    while (first[b + 1] <= lo) ++b;
+    for (size_t c = b; c < tiles.size() && first[c] < hi; ++c) {
+      if (tiles[c] == 0 || (first[c] >= lo && first[c + 1] <= hi)) continue;
+      const int s = p.slot(r, first[c]);
+      CHECK(s >= 0 && s < 2 * most);
+      CHECK(slots.insert(s).second);
+      written.insert({c, s});
+    }
+  }
+  size_t read = 0;
+  for (size_t c = 0; c < tiles.size(); ++c) {
+    if (tiles[c] == 0) continue;
+    const int r0 = p.of(first[c]), r1 = p.of(first[c + 1] - 1);
+    if (r0 == r1) continue;
+    for (int r = r0; r <= r1; ++r, ++read) CHECK(written.count({c, p.slot(r, first[c])}) == 1);
+  }
+  CHECK(read == written.size());
+}
+
+int main() {
+  std::mt19937 rng(1);
+  for (int i = 0; i < 4000; ++i) {
+    std::vector<int64_t> t(1 + rng() % (i % 4 ? 20 : 900));
+    for (auto& v : t) v = rng() % 3 == 0 ? 0 : 1 + rng() % (1 << rng() % 14);
+    check(t, 1 + static_cast<int>(rng() % 1200), 1 + static_cast<int>(rng() % 4));
+  }
+  check({(1ll << 32) - 1}, 1184, 2);
+  check({1, (1ll << 32) - 3, 1}, 1184, 2);
+  check({0, 0, 1, 0}, 148, 2);
+  check({0}, 148, 2);
+  std::printf("kv_plan_test: ok\n");
+}

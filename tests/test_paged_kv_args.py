@@ -53,6 +53,7 @@ BAD_ATTENTION = {
     "blocks shape": (lambda a: dict(blocks=torch.zeros(2, 1, 1, dtype=torch.int32)), "blocks must be"),
     "out type": (lambda a: dict(out=torch.zeros(a["q"].shape)), "out must be"),
     "out order": (lambda a: dict(out=wide(a["q"])), "out must be"),
+    "out address": (lambda a: dict(out=torch.zeros(2 * 8 * 64 + 1, dtype=torch.bfloat16)[1:].view(2, 8, 64)), "4-byte"),
     "out is q": (lambda a: dict(out=a["q"]), "overlap"),
     "gradient": (lambda a: dict(q=a["q"].clone().requires_grad_()), "no gradient"),
     "device": (lambda a: {}, "CUDA device"),
@@ -78,6 +79,10 @@ def test_attention_refuses_too_many_requests_and_tokens():
         ops.paged_kv_attention(q.expand(9000, -1, -1), kv, table.expand(9000, -1), lens.expand(9000))
     with pytest.raises(ValueError, match="too wide"):
         ops.paged_kv_attention(q, kv, table[:, :1].expand(1, 2**27), lens)
+    with pytest.raises(ValueError, match="too large"):
+        ops.paged_kv_attention(q.expand(64, -1, -1), kv, table[:, :1].expand(64, 2**26 - 1), lens.expand(64))
+    with pytest.raises(ValueError, match="a block"):
+        ops.paged_kv_evict(torch.zeros(table.shape), table, lens, 4, block_size=65537)
 
 
 def test_bounds_refuses(good):
@@ -121,3 +126,16 @@ def test_evict_refuses(good):
                         (dict(budget=2, sink=2), "at least sink"), (dict(block_size=0), "block_size"), ({}, "CUDA device")):
         with pytest.raises(ValueError, match=why):
             call(**change)
+
+
+def test_a_query_that_splits_pairs_is_copied(good):
+    from pcie_pool_b200.ops.paged_kv import _query
+
+    q = good["q"]
+    odd = torch.zeros(q.numel() + 1, dtype=q.dtype)[1:].view(q.shape).copy_(q)
+    spread = torch.zeros(*q.shape, 2, dtype=q.dtype)[..., 0].copy_(q)
+    rows = torch.zeros(2, 8, 65, dtype=q.dtype)[..., :64].copy_(q)
+    for x in (odd, spread, rows):
+        got = _query(x, q.device, q.dtype, 64, 2, 2)
+        assert got.data_ptr() % 4 == 0 and got.is_contiguous() and torch.equal(got, q)
+    assert _query(q, q.device, q.dtype, 64, 2, 2) is q
