@@ -439,55 +439,73 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 }
 
 // Adds up what the ranges left of a request that was cut: a CTA for each query
-// head, its warps take the parts in turn.  Requests without tokens get zeros.
-constexpr int kJoinWarps = 4;
+// head, its warps take four parts at a time.  Requests without tokens get zeros.
+constexpr int kJoinWarps = 8, kJoinParts = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ KvAttention a,
                                                                          const __grid_constant__ Work w) {
-  __shared__ float sum_o[kJoinWarps][256], sum_m[kJoinWarps], sum_l[kJoinWarps];
+  __shared__ __align__(16) float sum_o[kJoinWarps][256];
+  __shared__ float sum_m[kJoinWarps], sum_l[kJoinWarps];
   const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int D = a.kv.dim;
-  wait_for_parent();
-  const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
+  const int D = a.kv.dim, G = a.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
+  const int group = h / G * per_head + h % G / kRowGroup, row = h % G % kRowGroup;
   T* out = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.heads + h) * D;
   float* lse = a.lse + static_cast<long long>(b) * a.heads + h;
+  wait_for_parent();
+  const uint32_t f0 = w.first[b], f1 = w.first[b + 1], tiles = w.first[a.req.requests];
   if (f0 == f1) {
     for (int d = 2 * threadIdx.x; d < D; d += 2 * blockDim.x) *reinterpret_cast<uint32_t*>(out + d) = 0u;
     if (threadIdx.x == 0) *lse = -INFINITY;
     return;
   }
-  const KvPlan plan = KvPlan::make(w.first[a.req.requests], w.most_ranges, kLeastTiles);
+  const KvPlan plan = KvPlan::make(tiles, w.most_ranges, kLeastTiles);
   const int r0 = plan.of(f0), r1 = plan.of(f1 - 1);
   if (r0 == r1) return;  // finished where it was computed
-  const int G = a.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
-  const int group = h / G * per_head + h % G / kRowGroup, row = h % G % kRowGroup;
+  // the first part may lie in its range's second place, the others lie in the first
+  const long long base = static_cast<long long>(group) * w.rows + row, step = static_cast<long long>(w.groups) * w.rows;
+  const int slot0 = plan.slot(r0, f0);
   float m = -INFINITY, l = 0.f, o[8] = {};
-  for (int r = r0 + warp; r <= r1; r += kJoinWarps) {
-    const long long at = (static_cast<long long>(plan.slot(r, f0)) * w.groups + group) * w.rows + row;
-    const float2 ml = w.part_ml[at];
-    float4 v[2];
+  for (int r = r0 + warp * kJoinParts; r <= r1; r += kJoinWarps * kJoinParts) {
+    float2 ml[kJoinParts];
+    float4 v[kJoinParts][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (i * 128 + lane * 4 < D) v[i] = *reinterpret_cast<const float4*>(w.part_o + at * D + i * 128 + lane * 4);
-    const float now = fmaxf(m, ml.x), ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref), p = ex2(ml.x - ref);
-    m = now;
-    l = l * c + ml.y * p;
+    for (int k = 0; k < kJoinParts; ++k) {
+      const long long at = base + step * (r + k == r0 ? slot0 : 2 * (r + k));
+      ml[k] = make_float2(-INFINITY, 0.f);
+      v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r + k <= r1) {
+        ml[k] = w.part_ml[at];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (i * 128 + lane * 4 < D) {
-        o[4 * i] = o[4 * i] * c + v[i].x * p;
-        o[4 * i + 1] = o[4 * i + 1] * c + v[i].y * p;
-        o[4 * i + 2] = o[4 * i + 2] * c + v[i].z * p;
-        o[4 * i + 3] = o[4 * i + 3] * c + v[i].w * p;
+        for (int i = 0; i < 2; ++i)
+          if (i * 128 + lane * 4 < D) v[k][i] = *reinterpret_cast<const float4*>(w.part_o + at * D + i * 128 + lane * 4);
       }
+    }
+    float now = m;
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) now = fmaxf(now, ml[k].x);
+    const float ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref);
+    m = now;
+    l *= c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= c;
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) {
+      const float p = ex2(ml[k].x - ref);
+      l += ml[k].y * p;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        o[4 * i] += v[k][i].x * p;
+        o[4 * i + 1] += v[k][i].y * p;
+        o[4 * i + 2] += v[k][i].z * p;
+        o[4 * i + 3] += v[k][i].w * p;
+      }
+    }
   }
   if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = i / 4 * 128 + lane * 4 + i % 4;
-    if (d < D) sum_o[warp][d] = o[i];
-  }
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<float4*>(&sum_o[warp][i * 128 + lane * 4]) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
   __syncthreads();
   float top = -INFINITY, total = 0.f, by[kJoinWarps];
 #pragma unroll

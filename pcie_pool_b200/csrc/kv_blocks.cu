@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Pag
 // warp takes eight blocks of one key head at a time (their loads are in flight
 // together, and their sums are reduced together); it reads `kReach` channels of
 // lower and upper bounds with 8 bytes a lane each.  The bounds' bytes bound it.
-constexpr int kScoreWarps = 8, kScoreBlocks = 32, kTogether = 8, kReach = 128;
+constexpr int kScoreWarps = 8, kScoreBlocks = 16, kTogether = 8, kReach = 128;
 
 template <typename T, int PARTS>  // PARTS: dim / kReach, rounded up
 __global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_constant__ KvSelect s) {
@@ -226,6 +227,23 @@ struct Counter {
   }
 };
 
+// Keys of a row of values whose table entries lie in [0, pages).
+struct ValueKey {
+  const float* value;
+  const int* table;
+  int pages, n, sink, recent;
+
+  struct Raw {
+    float value;
+    int page;
+  };
+  __device__ Raw read(int j) const { return {value[j], table[j]}; }
+  __device__ unsigned make(int j, Raw r) const {
+    if (r.page < 0 || r.page >= pages) return 0u;
+    return j < sink || j >= n - recent ? 0xffffffffu : key_of(r.value);
+  }
+};
+
 struct Border {
   unsigned above;  // every key above it is taken
   int ties;        // and so many equal to it, from the lowest index
@@ -239,11 +257,15 @@ struct Row {
   Counter<THREADS> counter;
   unsigned keys[ITEMS];
 
+  // All of a thread's values are on their way before the first is looked at.
   __device__ void load(int base) {
+    decltype(key.read(0)) raw[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) raw[i] = key.read(min(base + static_cast<int>(threadIdx.x) * ITEMS + i, n - 1));
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int j = base + threadIdx.x * ITEMS + i;
-      keys[i] = j < n ? key(j) : 0u;
+      keys[i] = j < n ? key.make(j, raw[i]) : 0u;
     }
   }
   __device__ int at_least(unsigned c) {
@@ -257,6 +279,7 @@ struct Row {
   }
   // Border of the `want` highest.
   __device__ Border border(int want) {
+    if (n == 0) return {0xffffffffu, 0};
     if (n <= kChunk) load(0);
     want = min(want, at_least(1u));
     if (want == 0) return {0xffffffffu, 0};
@@ -323,12 +346,7 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
   const int* table = s.req.table + b * s.req.table_stride;
   int* out = s.out + static_cast<long long>(blockIdx.x) * s.keep;
   wait_for_parent();
-  auto key = [&](int j) -> unsigned {
-    const int page = table[j];
-    if (page < 0 || page >= s.pages) return 0u;
-    return j < s.sink || j >= n - s.recent ? 0xffffffffu : key_of(score[j]);
-  };
-  Row<THREADS, ITEMS, decltype(key)> row{key, n, {scratch}};
+  Row<THREADS, ITEMS, ValueKey> row{{score, table, s.pages, n, s.sink, s.recent}, n, {scratch}};
   const Border e = row.border(s.keep);
   const int done = row.emit(e, [&](int j, int at) { out[at] = j; }, [](int, int) {});
   for (int j = done + threadIdx.x; j < s.keep; j += THREADS) out[j] = -1;
@@ -342,11 +360,7 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const __grid_constant__ 
   const float* mass = e.mass + b * e.mass_stride;
   const int* table = e.req.table + b * e.req.table_stride;
   const long long at0 = static_cast<long long>(b) * width;
-  auto key = [&](int j) -> unsigned {
-    if (table[j] < 0) return 0u;
-    return j < e.sink || j >= n - e.recent ? 0xffffffffu : key_of(mass[j]);
-  };
-  Row<THREADS, ITEMS, decltype(key)> row{key, n, {scratch}};
+  Row<THREADS, ITEMS, ValueKey> row{{mass, table, INT_MAX, n, e.sink, e.recent}, n, {scratch}};
   const Border border = row.border(e.budget);
   int tokens = 0;
   const int kept = row.emit(
