@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "device_utils.cuh"
@@ -34,6 +35,7 @@ namespace {
 
 constexpr int kTile = 16;      // tokens of a step; the mass is gathered by tiles
 constexpr int kLeastTiles = 2; // of a range: shorter ones cost more to join than they save
+constexpr int kMostRequests = 4096;
 constexpr int kRowGroup = 16;  // query heads of one warp at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
   __shared__ uint32_t valid_of[S::kWarps][S::kStages];
   uint32_t* first = reinterpret_cast<uint32_t*>(smem + S::kRingBytes);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int D = a.kv.dim, bs = a.kv.block, G = a.heads / a.kv.kv_heads, n = a.req.requests;
+  const int D = a.kv.dim, bs = a.kv.block, G = a.q.heads / a.kv.kv_heads, n = a.req.requests;
   launch_dependents();
   if (D < DP)  // what the copies leave of a row stays zero
     for (int i = threadIdx.x; i < S::kRingBytes / 16; i += blockDim.x)
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
         b = b < 0 ? request_of(first, n, tile) : b + 1;
         while (first[b + 1] <= tile) ++b;
         end = first[b + 1];
-        const T* qp = static_cast<const T*>(a.q) + b * a.q_stride + (g * G + row0) * a.q_head_stride;
+        const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
             q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
                           ? 0u
-                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q_head_stride + d);
+                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
           }
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
           const int row = lane / 4 + 8 * x;
           if ((lane & 3) == 0 && row < rows)
-            w.z[(static_cast<long long>(b) * w.max_tiles + (tile - first[b])) * a.heads + g * G + row0 + row] = at + lg2(sum);
+            w.z[(static_cast<long long>(b) * w.max_tiles + (tile - first[b])) * a.q.heads + g * G + row0 + row] = at + lg2(sum);
         }
       }
       if (__any_sync(0xffffffffu, grew)) {
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
           const float by = sum == 0.f ? 0.f : 1.f / sum;
           if ((lane & 3) == 0) {
             if (whole)
-              a.lse[static_cast<long long>(b) * a.heads + h] = sum == 0.f ? -INFINITY : (m[x] + lg2(sum)) * kLn2;
+              a.lse[static_cast<long long>(b) * a.q.heads + h] = sum == 0.f ? -INFINITY : (m[x] + lg2(sum)) * kLn2;
             else
               w.part_ml[at] = make_float2(m[x], sum);
           }
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
             const float u = PACKED ? o[i][0] + o[i][2] : o[i][2 * x], v = PACKED ? o[i][1] + o[i][3] : o[i][2 * x + 1];
             if (d < D) {
               if (whole)
-                *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (static_cast<long long>(b) * a.heads + h) * D + d) =
+                *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (static_cast<long long>(b) * a.q.heads + h) * D + d) =
                     Type<T>::pack(sum == 0.f ? 0.f : u * by, sum == 0.f ? 0.f : v * by);
               else
                 *reinterpret_cast<float2*>(w.part_o + at * D + d) = make_float2(u, v);
@@ -447,11 +449,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
                                                                          const __grid_constant__ Work w) {
   __shared__ __align__(16) float sum_o[kJoinWarps][256];
   __shared__ float sum_m[kJoinWarps], sum_l[kJoinWarps];
-  const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int D = a.kv.dim, G = a.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
+  const int b = blockIdx.x / a.q.heads, h = blockIdx.x % a.q.heads, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int D = a.kv.dim, G = a.q.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
   const int group = h / G * per_head + h % G / kRowGroup, row = h % G % kRowGroup;
-  T* out = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.heads + h) * D;
-  float* lse = a.lse + static_cast<long long>(b) * a.heads + h;
+  T* out = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.q.heads + h) * D;
+  float* lse = a.lse + static_cast<long long>(b) * a.q.heads + h;
   wait_for_parent();
   const uint32_t f0 = w.first[b], f1 = w.first[b + 1], tiles = w.first[a.req.requests];
   if (f0 == f1) {
@@ -535,10 +537,10 @@ __global__ void __launch_bounds__(128) mass_kernel(const __grid_constant__ KvAtt
   if (j >= (len + a.kv.block - 1) / a.kv.block) return;
   const int per = a.kv.block / kTile, t0 = j * per, t1 = min(t0 + per, (len + kTile - 1) / kTile);
   float sum = 0.f;
-  for (int h = lane; h < a.heads; h += 32) {
-    const float total = a.lse[static_cast<long long>(b) * a.heads + h] * kLog2e;
+  for (int h = lane; h < a.q.heads; h += 32) {
+    const float total = a.lse[static_cast<long long>(b) * a.q.heads + h] * kLog2e;
     for (int t = t0; t < t1; ++t) {
-      const float v = w.z[(static_cast<long long>(b) * w.max_tiles + t) * a.heads + h];
+      const float v = w.z[(static_cast<long long>(b) * w.max_tiles + t) * a.q.heads + h];
       sum += v == -INFINITY ? 0.f : ex2(v - total);
     }
   }
@@ -551,30 +553,30 @@ int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
 
 // The workspace's parts behind `base`; returns its size.
-uint64_t lay_out(const KvAttention& a, int sms, void* base, Work& w) {
-  const int G = a.heads / a.kv.kv_heads, warps = sms * (padded(a.kv.dim) == 256 ? Shape<256>::kWarps : Shape<128>::kWarps);
-  w.groups = a.kv.kv_heads * ((G + kRowGroup - 1) / kRowGroup);
+uint64_t lay_out(int requests, int width, int block, int heads, int kv_heads, int dim, bool mass, int sms, void* base,
+                 Work& w) {
+  const int G = heads / kv_heads, warps = sms * (padded(dim) == 256 ? Shape<256>::kWarps : Shape<128>::kWarps);
+  w.groups = kv_heads * ((G + kRowGroup - 1) / kRowGroup);
   w.rows = G <= 8 ? 8 : 16;
   w.most_ranges = warps / w.groups > 0 ? warps / w.groups : 1;
-  w.max_tiles = static_cast<int>((static_cast<int64_t>(a.req.width) * a.kv.block + kTile - 1) / kTile);
+  w.max_tiles = static_cast<int>((static_cast<int64_t>(width) * block + kTile - 1) / kTile);
   const uint64_t parts = 2ull * w.most_ranges * w.groups * w.rows;
   uint8_t* p = static_cast<uint8_t*>(base);
   uint64_t at = 0;
   w.part_o = reinterpret_cast<float*>(p + at);
-  at += up(parts * a.kv.dim * 4);
+  at += up(parts * dim * 4);
   w.part_ml = reinterpret_cast<float2*>(p + at);
   at += up(parts * 8);
   w.first = reinterpret_cast<uint32_t*>(p + at);
-  at += up((a.req.requests + 1ull) * 4);
-  w.z = a.mass ? reinterpret_cast<float*>(p + at) : nullptr;
-  if (a.mass) at += up(uint64_t(a.req.requests) * w.max_tiles * a.heads * 4);
+  at += up((requests + 1ull) * 4);
+  w.z = mass ? reinterpret_cast<float*>(p + at) : nullptr;
+  if (mass) at += up(uint64_t(requests) * w.max_tiles * heads * 4);
   return at;
 }
 
-cudaError_t sm_count(int* sms) {
-  int device = 0;
-  cudaError_t rc = cudaGetDevice(&device);
-  return rc != cudaSuccess ? rc : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+cudaError_t sm_count(int* sms, int* device) {
+  cudaError_t rc = cudaGetDevice(device);
+  return rc != cudaSuccess ? rc : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *device);
 }
 
 // A kernel that may be resident before the one ahead of it in the stream is done
@@ -595,42 +597,53 @@ cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaSt
 }
 
 template <typename T, int DP>
-cudaError_t launch(const KvAttention& a, const Work& w, int sms, cudaStream_t stream) {
+cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cudaStream_t stream) {
   const int smem = Shape<DP>::kRingBytes + (a.req.requests + 1) * 4, threads = Shape<DP>::kWarps * 32;
   auto kernel = w.rows == 8 ? attention_kernel<T, DP, true> : attention_kernel<T, DP, false>;
-  cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (rc != cudaSuccess) return rc;
+  static_assert(Shape<DP>::kRingBytes + (kMostRequests + 1) * 4 <= 230 * 1024, "more shared memory than an SM has");
+  static std::atomic<uint64_t> ready[2];  // devices that know the kernels' shared memory
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  cudaError_t rc = cudaSuccess;
+  if (!(ready[w.rows == 8].load(std::memory_order_relaxed) & bit)) {
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Shape<DP>::kRingBytes + (kMostRequests + 1) * 4);
+    if (rc != cudaSuccess) return rc;
+    ready[w.rows == 8].fetch_or(bit, std::memory_order_relaxed);
+  }
   kernel<<<sms, threads, smem, stream>>>(a, w);
   rc = cudaGetLastError();
   if (rc != cudaSuccess) return rc;
-  return launch_after(attention_join_kernel<T>, dim3(a.req.requests * a.heads), kJoinWarps * 32, stream, a, w);
+  return launch_after(attention_join_kernel<T>, dim3(a.req.requests * a.q.heads), kJoinWarps * 32, stream, a, w);
 }
 
 template <typename T>
-cudaError_t launch(const KvAttention& a, const Work& w, int sms, cudaStream_t stream) {
+cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cudaStream_t stream) {
   switch (padded(a.kv.dim)) {
-    case 64: return launch<T, 64>(a, w, sms, stream);
-    case 128: return launch<T, 128>(a, w, sms, stream);
-    default: return launch<T, 256>(a, w, sms, stream);
+    case 64: return launch<T, 64>(a, w, sms, device, stream);
+    case 128: return launch<T, 128>(a, w, sms, device, stream);
+    default: return launch<T, 256>(a, w, sms, device, stream);
   }
 }
 
 }  // namespace
 
-uint64_t paged_kv_attention_work(const KvAttention& a) {
-  int sms = 0;
+uint64_t paged_kv_attention_work(int requests, int width, int block, int heads, int kv_heads, int dim, bool mass) {
+  int sms = 0, device = 0;
   Work w;
-  return sm_count(&sms) == cudaSuccess ? lay_out(a, sms, nullptr, w) : 0;
+  if (sm_count(&sms, &device) != cudaSuccess) return 0;
+  return lay_out(requests, width, block, heads, kv_heads, dim, mass, sms, nullptr, w);
 }
 
 cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream) {
   if (a.req.requests == 0) return cudaSuccess;
-  int sms = 0;
-  cudaError_t rc = sm_count(&sms);
+  if (a.req.requests > kMostRequests) return cudaErrorInvalidValue;
+  int sms = 0, device = 0;
+  cudaError_t rc = sm_count(&sms, &device);
   if (rc != cudaSuccess) return rc;
   Work w;
-  lay_out(a, sms, a.work, w);
-  rc = a.kv.type == kKvBf16 ? launch<__nv_bfloat16>(a, w, sms, stream) : launch<__half>(a, w, sms, stream);
+  lay_out(a.req.requests, a.req.width, a.kv.block, a.q.heads, a.kv.kv_heads, a.kv.dim, a.mass != nullptr, sms, a.work, w);
+  rc = a.kv.type == kKvBf16 ? launch<__nv_bfloat16>(a, w, sms, device, stream)
+                             : launch<__half>(a, w, sms, device, stream);
   if (rc == cudaSuccess && a.mass && a.req.width)
     rc = launch_after(mass_kernel, dim3((a.req.width + 3) / 4, a.req.requests), 128, stream, a, w);
   return rc;

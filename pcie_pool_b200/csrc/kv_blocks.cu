@@ -89,37 +89,76 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Pag
 // exponents, and the order of blocks does not hang on the order of summation.  A
 // warp takes eight blocks of one key head at a time (their loads are in flight
 // together, and their sums are reduced together); it reads `kReach` channels of
-// lower and upper bounds with 8 bytes a lane each.  The bounds' bytes bound it.
+// lower and upper bounds with 8 bytes a lane each.
+//
+// The conversion to 64 bits (a sixteenth of the rate of a product) is left out:
+// the bits of a bf16 or fp16 value, moved to where a double keeps its exponent and
+// mantissa, are that value times a power of two, subnormals and zero included.
+// A and B carry half of that power, and the sum gets the other half back.  Infinities
+// and values that are not a number do not move so; a row that has one (0 * x tells)
+// is summed again with converted values.
 constexpr int kScoreWarps = 8, kScoreBlocks = 16, kTogether = 8, kReach = 128;
+
+template <typename T>
+struct Moved;
+template <>
+struct Moved<__nv_bfloat16> {  // exponent of 8 bits, bias 127: 2^(127 - 1023)
+  static constexpr int kShift = 3;
+  static constexpr uint32_t kMask = 0x8fffe000u;
+  static constexpr double kHalf = 0x1p448;
+};
+template <>
+struct Moved<__half> {  // exponent of 5 bits, bias 15: 2^(15 - 1023)
+  static constexpr int kShift = 6;
+  static constexpr uint32_t kMask = 0x81fffc00u;
+  static constexpr double kHalf = 0x1p504;
+};
+template <typename T>
+__device__ __forceinline__ double move(uint32_t pair, int which) {
+  const int v = static_cast<int>(which ? pair : pair << 16);
+  return __hiloint2double((v >> Moved<T>::kShift) & Moved<T>::kMask, 0);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t zero_unless_special(uint32_t pair, uint32_t so_far) {
+  using P = typename Pair<T>::type;
+  const P zero = {T(0.f), T(0.f)};
+  P r = __hfma2(reinterpret_cast<P&>(pair), zero, reinterpret_cast<P&>(so_far));
+  return reinterpret_cast<uint32_t&>(r);
+}
 
 template <typename T, int PARTS>  // PARTS: dim / kReach, rounded up
 __global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_constant__ KvSelect s) {
-  const int b = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32, G = s.heads / s.kv_heads;
+  const int b = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32, G = s.q.heads / s.kv_heads;
   launch_dependents();
-  const int n = (length_of(s.req, s.block, b) + s.block - 1) / s.block;
   const int from = blockIdx.x * kScoreBlocks;
-  if (from >= n) return;
-  const int batches = (min(kScoreBlocks, n - from) + kTogether - 1) / kTogether;
   const int* table = s.req.table + b * s.req.table_stride;
+  const int len = s.req.lens[b];
+  // looked up before the length is known, so that the two loads wait together
+  int pages = lane < kScoreBlocks && from + lane < s.req.width ? table[from + lane] : -1;
+  const int n = static_cast<int>((max(0ll, min(static_cast<long long>(len), static_cast<long long>(s.req.width) * s.block)) +
+                                  s.block - 1) / s.block);
+  if (from >= n) return;
+  if (from + lane >= n || pages >= s.pages) pages = -1;
+  const int batches = (min(kScoreBlocks, n - from) + kTogether - 1) / kTogether;
   double above[PARTS][4], below[PARTS][4];
   uint32_t above_on[PARTS][2], below_on[PARTS][2];  // channels that count: 0 * inf shall be nothing
+  const int row_values = s.kv_heads * 2 * s.dim;
   int have = -1;
   for (int unit = warp; unit < s.kv_heads * batches; unit += kScoreWarps) {
-    const int g = unit % s.kv_heads, j0 = from + unit / s.kv_heads * kTogether;
-    int page = lane < kTogether && j0 + lane < n ? table[j0 + lane] : -1;
-    if (page >= s.pages) page = -1;
+    const int g = unit % s.kv_heads, first = unit / s.kv_heads * kTogether, j0 = from + first;
+    const T* bounds = static_cast<const T*>(s.bounds) + g * 2 * s.dim + lane * 4;
     uint2 lo[kTogether][PARTS], hi[kTogether][PARTS];
 #pragma unroll
     for (int i = 0; i < kTogether; ++i) {
-      const int at = __shfl_sync(0xffffffffu, page, i);
-      const T* row = static_cast<const T*>(s.bounds) + (static_cast<long long>(max(at, 0)) * s.kv_heads + g) * 2 * s.dim;
+      const int page = __shfl_sync(0xffffffffu, pages, first + i);
+      const bool there = page >= 0;
+      const T* row = bounds + static_cast<long long>(page) * row_values;
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-        const int d = p * kReach + lane * 4;
         lo[i][p] = hi[i][p] = make_uint2(0, 0);
-        if (at >= 0 && d < s.dim) {
-          lo[i][p] = *reinterpret_cast<const uint2*>(row + d);
-          hi[i][p] = *reinterpret_cast<const uint2*>(row + s.dim + d);
+        if (there && p * kReach + lane * 4 < s.dim) {
+          lo[i][p] = *reinterpret_cast<const uint2*>(row + p * kReach);
+          hi[i][p] = *reinterpret_cast<const uint2*>(row + s.dim + p * kReach);
         }
       }
     }
@@ -127,42 +166,75 @@ __global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_co
       have = g;
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) above[p][i] = below[p][i] = 0;
+        double up[4] = {}, down[4] = {};
         const int d = p * kReach + lane * 4;
         if (d < s.dim) {
-          const T* q = static_cast<const T*>(s.q) + b * s.q_stride + g * G * s.q_head_stride + d;
-          for (int h = 0; h < G; ++h, q += s.q_head_stride) {
-            const float2 x = floats<T>(*reinterpret_cast<const uint32_t*>(q)), y = floats<T>(*reinterpret_cast<const uint32_t*>(q + 2));
-            const float v[4] = {x.x, x.y, y.x, y.y};
+          const T* q = static_cast<const T*>(s.q.base) + b * s.q.stride + g * G * s.q.head_stride + d;
+#pragma unroll 4
+          for (int h = 0; h < G; ++h, q += s.q.head_stride) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(q), y = *reinterpret_cast<const uint32_t*>(q + 2);
+            const float2 f = floats<T>(x), e = floats<T>(y);
+            const float v[4] = {f.x, f.y, e.x, e.y};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) (v[i] < 0.f ? below : above)[p][i] += v[i];
+            for (int i = 0; i < 4; ++i) {
+              const double w = v[i];
+              if (v[i] < 0.f)
+                down[i] += w;
+              else
+                up[i] += w;
+            }
           }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          above_on[p][i] = (above[p][2 * i] != 0 ? 0xffffu : 0u) | (above[p][2 * i + 1] != 0 ? 0xffff0000u : 0u);
-          below_on[p][i] = (below[p][2 * i] != 0 ? 0xffffu : 0u) | (below[p][2 * i + 1] != 0 ? 0xffff0000u : 0u);
+          above_on[p][i] = (up[2 * i] != 0 ? 0xffffu : 0u) | (up[2 * i + 1] != 0 ? 0xffff0000u : 0u);
+          below_on[p][i] = (down[2 * i] != 0 ? 0xffffu : 0u) | (down[2 * i + 1] != 0 ? 0xffff0000u : 0u);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) above[p][i] = up[i] * Moved<T>::kHalf, below[p][i] = down[i] * Moved<T>::kHalf;
       }
     }
     double sum[kTogether];
+    uint32_t special = 0;
 #pragma unroll
     for (int i = 0; i < kTogether; ++i) {
       sum[i] = 0;
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-        const uint32_t l[2] = {lo[i][p].x, lo[i][p].y}, u[2] = {hi[i][p].x, hi[i][p].y};
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float2 top = floats<T>(most2<T>(l[x], u[x]) & above_on[p][x]);
-          const float2 low = floats<T>(least2<T>(l[x], u[x]) & below_on[p][x]);
-          sum[i] += above[p][2 * x] * top.x;
-          sum[i] += above[p][2 * x + 1] * top.y;
-          sum[i] += below[p][2 * x] * low.x;
-          sum[i] += below[p][2 * x + 1] * low.y;
-        }
+        const uint2 l = lo[i][p], u = hi[i][p];
+        hi[i][p] = make_uint2(most2<T>(l.x, u.x) & above_on[p][0], most2<T>(l.y, u.y) & above_on[p][1]);
+        lo[i][p] = make_uint2(least2<T>(l.x, u.x) & below_on[p][0], least2<T>(l.y, u.y) & below_on[p][1]);
+        special = zero_unless_special<T>(hi[i][p].x, zero_unless_special<T>(hi[i][p].y, special));
+        special = zero_unless_special<T>(lo[i][p].x, zero_unless_special<T>(lo[i][p].y, special));
+        sum[i] += above[p][0] * move<T>(hi[i][p].x, 0);
+        sum[i] += above[p][1] * move<T>(hi[i][p].x, 1);
+        sum[i] += above[p][2] * move<T>(hi[i][p].y, 0);
+        sum[i] += above[p][3] * move<T>(hi[i][p].y, 1);
+        sum[i] += below[p][0] * move<T>(lo[i][p].x, 0);
+        sum[i] += below[p][1] * move<T>(lo[i][p].x, 1);
+        sum[i] += below[p][2] * move<T>(lo[i][p].y, 0);
+        sum[i] += below[p][3] * move<T>(lo[i][p].y, 1);
       }
+    }
+    double by = Moved<T>::kHalf;
+    if (__any_sync(0xffffffffu, special & 0x7fff7fffu)) {
+      by = 1 / Moved<T>::kHalf;
+#pragma unroll 1
+      for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+          const uint2 u = PARTS > 1 && p ? hi[i][PARTS - 1] : hi[i][0], l = PARTS > 1 && p ? lo[i][PARTS - 1] : lo[i][0];
+          const float2 v[4] = {floats<T>(u.x), floats<T>(u.y), floats<T>(l.x), floats<T>(l.y)};
+          if (p == 0) sum[i] = 0;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const double a0 = PARTS > 1 && p ? above[PARTS - 1][2 * x] : above[0][2 * x],
+                         a1 = PARTS > 1 && p ? above[PARTS - 1][2 * x + 1] : above[0][2 * x + 1],
+                         b0 = PARTS > 1 && p ? below[PARTS - 1][2 * x] : below[0][2 * x],
+                         b1 = PARTS > 1 && p ? below[PARTS - 1][2 * x + 1] : below[0][2 * x + 1];
+            sum[i] += a0 * v[x].x + a1 * v[x].y + (b0 * v[2 + x].x + b1 * v[2 + x].y);
+          }
+        }
     }
     // halve the eight sums while the lanes are added: lane bits 4, 3 and 2 choose the block
 #pragma unroll
@@ -177,15 +249,19 @@ __global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_co
     sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
     const int j = j0 + (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
     if ((lane & 3) == 0 && j < n)
-      s.scores[(static_cast<long long>(b) * s.kv_heads + g) * s.req.width + j] = static_cast<float>(sum[0]);
+      s.scores[(static_cast<long long>(b) * s.kv_heads + g) * s.req.width + j] = static_cast<float>(sum[0] * by);
   }
 }
 
 // ---- the highest of a row --------------------------------------------------------------
-// A CTA for each row.  A thread holds ITEMS neighbours as unsigned keys in the order
-// of the values; the border is found bit by bit from the top, counting the keys
-// above it, and the row is written in order by a scan over the threads.  Rows longer
-// than THREADS * ITEMS are read again in every pass.
+// A CTA for each row.  A thread holds every THREADS-th value as an unsigned key in
+// the order of the values.  The border is found by counting: the keys between the
+// least and the highest that are still in question fall into 2048 bins of the
+// highest bits in which they differ, the bin that holds the border is what is in
+// question next, three times at most.  The row is then written in order by the
+// counts of every warp's share of it.  Rows longer than THREADS * ITEMS are read
+// again in every pass.  Latency bounds it: of the reads, some ten barriers, and the
+// atomics of keys that fall together.
 
 // Not a number is the lowest value, both zeros are equal.  0 is left for what cannot
 // be taken, all ones for what must be.
@@ -194,38 +270,6 @@ __device__ __forceinline__ unsigned key_of(float v) {
   const unsigned u = __float_as_uint(v == 0.f ? 0.f : v);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-
-template <int THREADS>
-struct Counter {
-  static constexpr int kWarps = THREADS / 32;
-  int (*scratch)[32];  // two rows in turn, so that one barrier a count is enough
-  int turn = 0;
-
-  __device__ int sum(int v) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    int* row = scratch[turn ^= 1];
-    if (threadIdx.x % 32 == 0) row[threadIdx.x / 32] = v;
-    __syncthreads();
-    const int lane = threadIdx.x % 32;
-    return __reduce_add_sync(0xffffffffu, lane < kWarps ? row[lane] : 0);
-  }
-  // Sum of the lower threads' v; `total` of all.
-  __device__ int before(int v, int& total) {
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    int upto = v;
-#pragma unroll
-    for (int x = 1; x < 32; x *= 2) {
-      const int u = __shfl_up_sync(0xffffffffu, upto, x);
-      if (lane >= x) upto += u;
-    }
-    int* row = scratch[turn ^= 1];
-    if (lane == 31) row[warp] = upto;
-    __syncthreads();
-    const int w = lane < kWarps ? row[lane] : 0;
-    total = __reduce_add_sync(0xffffffffu, w);
-    return upto - v + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
-  }
-};
 
 // Keys of a row of values whose table entries lie in [0, pages).
 struct ValueKey {
@@ -251,119 +295,243 @@ struct Border {
 
 template <int THREADS, int ITEMS, typename Key>
 struct Row {
-  static constexpr int kChunk = THREADS * ITEMS;
+  static constexpr int kChunk = THREADS * ITEMS, kWarps = THREADS / 32, kShares = ITEMS * kWarps;
+  static constexpr int kBinBits = 11, kBins = 1 << kBinBits, kOwn = kBins / THREADS;
+  static constexpr unsigned kMust = 0xffffffffu;
+  struct Shared {
+    int bins[kBins];
+    int sums[kWarps];
+    unsigned least[kWarps], most[kWarps];
+    int must[kWarps];
+    int found[3];            // the border's bin, the keys above it, the keys in it
+    int share[kShares + 1];  // of a chunk, in its order: item by item, warp by warp
+  };
   Key key;
   int n;
-  Counter<THREADS> counter;
+  Shared& shared;
   unsigned keys[ITEMS];
+  int taken = 0, left = 0;
+
+  __device__ Row(const Key& k, int n_, Shared& s) : key(k), n(n_), shared(s) {}
 
   // All of a thread's values are on their way before the first is looked at.
   __device__ void load(int base) {
-    decltype(key.read(0)) raw[ITEMS];
+    typename Key::Raw raw[ITEMS];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) raw[i] = key.read(min(base + static_cast<int>(threadIdx.x) * ITEMS + i, n - 1));
+    for (int i = 0; i < ITEMS; ++i) raw[i] = key.read(min(base + i * THREADS + static_cast<int>(threadIdx.x), n - 1));
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int j = base + threadIdx.x * ITEMS + i;
+      const int j = base + i * THREADS + threadIdx.x;
       keys[i] = j < n ? key.make(j, raw[i]) : 0u;
     }
   }
-  __device__ int at_least(unsigned c) {
-    int m = 0;
+  // f(key) for every key of the row.
+  template <typename F>
+  __device__ void each(F f) {
     for (int base = 0; base < n; base += kChunk) {
       if (n > kChunk) load(base);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) m += keys[i] >= c;
+      for (int i = 0; i < ITEMS; ++i) f(keys[i]);
     }
-    return counter.sum(m);
   }
-  // Border of the `want` highest.
+  // Border of the `want` highest; those that must be taken are no more than that.
   __device__ Border border(int want) {
-    if (n == 0) return {0xffffffffu, 0};
+    if (n == 0) return {kMust, 0};
     if (n <= kChunk) load(0);
-    want = min(want, at_least(1u));
-    if (want == 0) return {0xffffffffu, 0};
-    unsigned t = 0;
-    int over = 0;  // keys above all that begin like t
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned c = t | 1u << bit;
-      const int m = at_least(c);
-      if (m == want) return {c - 1, 0};
-      if (m > want)
-        t = c;
-      else
-        over = m;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    unsigned least = kMust, most = 0;
+    int can = 0, must = 0;
+    each([&](unsigned k) {
+      must += k == kMust;
+      if (k != 0 && k != kMust) {
+        ++can;
+        least = min(least, k);
+        most = max(most, k);
+      }
+    });
+    can = __reduce_add_sync(0xffffffffu, can);
+    must = __reduce_add_sync(0xffffffffu, must);
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) shared.sums[warp] = can, shared.must[warp] = must, shared.least[warp] = least, shared.most[warp] = most;
+    for (int i = threadIdx.x; i < kBins; i += THREADS) shared.bins[i] = 0;
+    __syncthreads();
+    can = must = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      can += shared.sums[w];
+      must += shared.must[w];
+      least = min(least, shared.least[w]);
+      most = max(most, shared.most[w]);
     }
-    return {t, want - over};
+    want -= must;
+    if (want >= can) return {0u, 0};
+    if (want <= 0) return {kMust - 1, 0};
+    while (true) {  // 0 < want < number of the keys in [least, most]
+      if (least == most) return {least, want};
+      const int shift = max(0, 32 - __clz(least ^ most) - kBinBits);
+      const unsigned low = least >> shift;
+      each([&](unsigned k) {
+        if (k >= least && k <= most && k != kMust) atomicAdd(&shared.bins[(k >> shift) - low], 1);
+      });
+      __syncthreads();
+      // from the highest bin down: thread t owns bins [kBins - (t + 1) kOwn, kBins - t kOwn)
+      int own[kOwn], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        own[i] = shared.bins[kBins - 1 - (threadIdx.x * kOwn + i)];
+        mine += own[i];
+      }
+      int upto = mine;
+#pragma unroll
+      for (int x = 1; x < 32; x *= 2) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += u;
+      }
+      if (lane == 31) shared.sums[warp] = upto;
+      __syncthreads();
+      int above = upto - mine;
+      for (int w = 0; w < warp; ++w) above += shared.sums[w];
+      if (above < want && above + mine >= want) {
+        int i = 0;
+#pragma unroll
+        for (int x = 0; x < kOwn - 1; ++x)
+          if (i == x && above + own[x] < want) {
+            above += own[x];
+            ++i;
+          }
+        shared.found[0] = kBins - 1 - (threadIdx.x * kOwn + i);
+        shared.found[1] = above;
+        shared.found[2] = shared.bins[kBins - 1 - (threadIdx.x * kOwn + i)];
+      }
+      __syncthreads();
+      const unsigned bin = low + shared.found[0];
+      want -= shared.found[1];
+      const unsigned from = max(least, bin << shift), to = min(most, (bin << shift) + ((1u << shift) - 1));
+      if (want == shared.found[2]) return {from - 1, 0};  // all of the bin; from > 0
+      least = from;
+      most = to;
+      for (int i = threadIdx.x; i < kBins; i += THREADS) shared.bins[i] = 0;
+      __syncthreads();
+    }
   }
-  // put(index, key, rank among the taken) for what is taken, leave(index, rank) for
-  // the others that could be; returns the number of the taken.
-  template <typename Put, typename Leave>
-  __device__ int emit(const Border& e, Put put, Leave leave) {
-    int ties = 0, done = 0, gone = 0;
+  // Before this thread's item i in the chunk: where `flag` holds, by the ballots in
+  // `votes` and the shares' sums.
+  __device__ int rank(unsigned vote, int i) const {
+    return shared.share[i * kWarps + threadIdx.x / 32] + __popc(vote & ((1u << threadIdx.x % 32) - 1));
+  }
+  // Turns the shares' counts into the numbers before them; returns their total.
+  __device__ int scan_shares() {
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      constexpr int kEach = (kShares + 31) / 32;
+      const int lane = threadIdx.x;
+      int v[kEach], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int at = lane * kEach + i;
+        v[i] = at < kShares ? shared.share[at] : 0;
+        mine += v[i];
+      }
+      int upto = mine;
+#pragma unroll
+      for (int x = 1; x < 32; x *= 2) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += u;
+      }
+      int before = upto - mine;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int at = lane * kEach + i;
+        if (at < kShares) shared.share[at] = before;
+        before += v[i];
+      }
+      if (lane == 31) shared.share[kShares] = upto;
+    }
+    __syncthreads();
+    return shared.share[kShares];
+  }
+  // put(index, rank among the taken) for what is taken, leave(index, rank) for the
+  // others that could be; sets the numbers of both.
+  template <bool LEAVE, typename Put, typename Leave>
+  __device__ void emit(const Border& e, Put put, Leave leave) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    int ties = 0;
+    taken = left = 0;
     for (int base = 0; base < n; base += kChunk) {
       if (n > kChunk) load(base);
-      int tie = 0, can = 0;
+      unsigned take[ITEMS];
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) tie += keys[i] == e.above && keys[i] != 0, can += keys[i] != 0;
-      int all_ties, all;
-      const int tie0 = ties + counter.before(tie, all_ties);
-      int take = 0, seen = tie0;
-      bool taken[ITEMS];
+      for (int i = 0; i < ITEMS; ++i) take[i] = __ballot_sync(0xffffffffu, keys[i] > e.above);
+      if (e.ties > 0) {
+        unsigned tie[ITEMS];
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        const bool equal = keys[i] == e.above && keys[i] != 0;
-        taken[i] = keys[i] > e.above || (equal && seen < e.ties);
-        seen += equal;
-        take += taken[i];
+        for (int i = 0; i < ITEMS; ++i) {
+          tie[i] = __ballot_sync(0xffffffffu, keys[i] == e.above && keys[i] != 0);
+          if (lane == 0) shared.share[i * kWarps + warp] = __popc(tie[i]);
+        }
+        const int all = scan_shares();
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+          take[i] |= __ballot_sync(0xffffffffu, (tie[i] >> lane & 1) && ties + rank(tie[i], i) < e.ties);
+        ties += all;
+        __syncthreads();
       }
-      int at = done + counter.before(take, all), all_gone;
-      int out = gone + counter.before(can - take, all_gone);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        const int j = base + threadIdx.x * ITEMS + i;
-        if (taken[i])
-          put(j, at++);
-        else if (keys[i] != 0)
-          leave(j, out++);
+      for (int i = 0; i < ITEMS; ++i)
+        if (lane == 0) shared.share[i * kWarps + warp] = __popc(take[i]);
+      const int all = scan_shares();
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        if (take[i] >> lane & 1) put(base + i * THREADS + static_cast<int>(threadIdx.x), taken + rank(take[i], i));
+      taken += all;
+      __syncthreads();
+      if (LEAVE) {
+        unsigned rest[ITEMS];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          rest[i] = __ballot_sync(0xffffffffu, keys[i] != 0) & ~take[i];
+          if (lane == 0) shared.share[i * kWarps + warp] = __popc(rest[i]);
+        }
+        const int others = scan_shares();
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+          if (rest[i] >> lane & 1) leave(base + i * THREADS + static_cast<int>(threadIdx.x), left + rank(rest[i], i));
+        left += others;
+        __syncthreads();
       }
-      ties += all_ties;
-      done += all;
-      gone += all_gone;
     }
-    left = gone;
-    return done;
   }
-  int left = 0;  // of the others
 };
 
 template <int THREADS, int ITEMS>
 __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ KvSelect s) {
-  __shared__ int scratch[2][32];
+  using Keys = Row<THREADS, ITEMS, ValueKey>;
+  __shared__ typename Keys::Shared shared;
   const int b = blockIdx.x / s.kv_heads;
   const int n = (length_of(s.req, s.block, b) + s.block - 1) / s.block;
   const float* score = s.scores + static_cast<long long>(blockIdx.x) * s.req.width;
   const int* table = s.req.table + b * s.req.table_stride;
   int* out = s.out + static_cast<long long>(blockIdx.x) * s.keep;
   wait_for_parent();
-  Row<THREADS, ITEMS, ValueKey> row{{score, table, s.pages, n, s.sink, s.recent}, n, {scratch}};
+  Keys row({score, table, s.pages, n, s.sink, s.recent}, n, shared);
   const Border e = row.border(s.keep);
-  const int done = row.emit(e, [&](int j, int at) { out[at] = j; }, [](int, int) {});
-  for (int j = done + threadIdx.x; j < s.keep; j += THREADS) out[j] = -1;
+  row.template emit<false>(e, [&](int j, int at) { out[at] = j; }, [](int, int) {});
+  for (int j = row.taken + threadIdx.x; j < s.keep; j += THREADS) out[j] = -1;
 }
 
 template <int THREADS, int ITEMS>
 __global__ void __launch_bounds__(THREADS) evict_kernel(const __grid_constant__ KvEvict e) {
-  __shared__ int scratch[2][32];
+  using Keys = Row<THREADS, ITEMS, ValueKey>;
+  __shared__ typename Keys::Shared shared;
   const int b = blockIdx.x, width = e.req.width, len = length_of(e.req, e.block, b);
   const int n = (len + e.block - 1) / e.block;
   const float* mass = e.mass + b * e.mass_stride;
   const int* table = e.req.table + b * e.req.table_stride;
   const long long at0 = static_cast<long long>(b) * width;
-  Row<THREADS, ITEMS, ValueKey> row{{mass, table, INT_MAX, n, e.sink, e.recent}, n, {scratch}};
+  Keys row({mass, table, INT_MAX, n, e.sink, e.recent}, n, shared);
   const Border border = row.border(e.budget);
   int tokens = 0;
-  const int kept = row.emit(
+  row.template emit<true>(
       border,
       [&](int j, int at) {
         e.new_table[at0 + at] = table[j];
@@ -374,25 +542,30 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const __grid_constant__ 
         e.evicted[at0 + at] = table[j];
         e.evicted_at[at0 + at] = j;
       });
-  for (int j = kept + threadIdx.x; j < width; j += THREADS) e.new_table[at0 + j] = -1, e.new_mass[at0 + j] = 0.f;
+  for (int j = row.taken + threadIdx.x; j < width; j += THREADS) e.new_table[at0 + j] = -1, e.new_mass[at0 + j] = 0.f;
   for (int j = row.left + threadIdx.x; j < width; j += THREADS) e.evicted[at0 + j] = -1, e.evicted_at[at0 + j] = -1;
-  tokens = row.counter.sum(tokens);
+  tokens = __reduce_add_sync(0xffffffffu, tokens);
+  if (threadIdx.x % 32 == 0) shared.sums[threadIdx.x / 32] = tokens;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    tokens = 0;
+    for (int w = 0; w < THREADS / 32; ++w) tokens += shared.sums[w];
     e.new_lens[b] = tokens;
     e.evicted_count[b] = row.left;
   }
 }
 
-// By the longest row there can be: fewer threads mean cheaper barriers.
+// By the longest row there can be: few threads with many values each, since what a
+// warp does besides its values costs more than they do.
 template <typename Launch>
 void for_width(int width, Launch launch) {
   using std::integral_constant;
   if (width <= 1024)
-    launch(integral_constant<int, 256>(), integral_constant<int, 4>());
+    launch(integral_constant<int, 128>(), integral_constant<int, 8>());
   else if (width <= 4096)
-    launch(integral_constant<int, 512>(), integral_constant<int, 8>());
+    launch(integral_constant<int, 256>(), integral_constant<int, 16>());
   else
-    launch(integral_constant<int, 1024>(), integral_constant<int, 16>());
+    launch(integral_constant<int, 512>(), integral_constant<int, 32>());
 }
 
 }  // namespace

@@ -22,7 +22,7 @@ struct PagedKv {
   int type = kKvBf16;
 };
 
-// The requests: their block table (int32, `width` entries a row) and lengths.
+// At most 4096 requests: their block table (int32, `width` entries a row) and lengths.
 // An entry outside [0, pages) is a block that is not resident: its tokens are
 // left out.  Lengths are cut to the table's width * block.
 struct KvRequests {
@@ -32,12 +32,18 @@ struct KvRequests {
   int requests = 0, width = 0;
 };
 
+// The new tokens' queries [requests, heads, dim]; the last dimension is contiguous,
+// pairs of values lie on 4-byte boundaries.
+struct KvQuery {
+  const void* base = nullptr;
+  int64_t stride = 0, head_stride = 0;
+  int heads = 0;
+};
+
 struct KvAttention {
   PagedKv kv;
   KvRequests req;
-  const void* q = nullptr;  // [requests, heads, dim]
-  int64_t q_stride = 0, q_head_stride = 0;
-  int heads = 0;
+  KvQuery q;
   float scale = 0.f;
   const int* blocks = nullptr;  // [requests, kv_heads, blocks_width] or null: every block
   int blocks_width = 0;
@@ -48,8 +54,8 @@ struct KvAttention {
   void* work = nullptr;    // paged_kv_attention_work() bytes
 };
 
-// Workspace bytes of a call on the current device (its pointers are not followed).
-uint64_t paged_kv_attention_work(const KvAttention& a);
+// Workspace bytes of a call on the current device.
+uint64_t paged_kv_attention_work(int requests, int width, int block, int heads, int kv_heads, int dim, bool mass);
 cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream);
 
 // Bounds [pages, kv_heads, 2, dim] (smallest, then largest key of each channel) of
@@ -60,9 +66,7 @@ cudaError_t paged_kv_bounds(const PagedKv& kv, const KvRequests& req, int new_to
 
 struct KvSelect {
   KvRequests req;
-  const void* q = nullptr;
-  int64_t q_stride = 0, q_head_stride = 0;
-  int heads = 0;
+  KvQuery q;
   const void* bounds = nullptr;  // [pages, kv_heads, 2, dim] contiguous
   int pages = 0, block = 0, kv_heads = 0, dim = 0, type = kKvBf16;
   int keep = 0, sink = 0, recent = 0;

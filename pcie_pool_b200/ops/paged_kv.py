@@ -34,7 +34,7 @@ from typing import NamedTuple
 
 from .._native import native
 
-MAX_REQUESTS = 8192
+MAX_REQUESTS = 4096
 MAX_DIM = 256
 MAX_BLOCK = 65536
 
@@ -45,76 +45,91 @@ def _torch():
     return torch
 
 
-def _need(ok: bool, why: str) -> None:
-    if not ok:
-        raise ValueError(why)
-
-
 def _int(v, name: str, least: int) -> int:
-    _need(isinstance(v, int) and not isinstance(v, bool) and least <= v < 2**31, f"{name} must be an integer >= {least}")
+    if not isinstance(v, int) or isinstance(v, bool) or not least <= v < 2**31:
+        raise ValueError(f"{name} must be an integer >= {least}")
     return v
 
 
-def _kv_type(dtype):
-    torch = _torch()
+def _kv_type(dtype, torch) -> int:
     if dtype == torch.bfloat16:
-        return native().KV_BF16
+        return 0
     if dtype == torch.float16:
-        return native().KV_FP16
+        return 1
     raise ValueError("the cache must be bf16 or fp16")
 
 
-def _cuda(device) -> None:
-    _need(device.type == "cuda", "the tensors must be on a CUDA device")
+def _runs(torch, *tensors) -> int:
+    """The stream that a call on these tensors runs on, as an integer; the last check of every call."""
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the paged-KV operators have no gradient: call them under torch.no_grad()")
+    t = tensors[0]
+    if not t.is_cuda:
+        raise ValueError("the tensors must be on a CUDA device")
+    # current_stream(t.device).cuda_stream without the Stream object: a tenth of the call's host time
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def _no_grad(*tensors) -> None:
-    if _torch().is_grad_enabled():
-        _need(not any(t.requires_grad for t in tensors), "the paged-KV operators have no gradient: call them under torch.no_grad()")
-
-
-def _requests(block_table, context_lens, device, block: int):
-    """Checked ``KvRequests`` of a table and its lengths."""
-    torch = _torch()
-    _need(block_table.dim() == 2 and block_table.dtype == torch.int32, "block_table must be int32 [requests, blocks]")
+def _requests(torch, block_table, context_lens, device: int, block: int):
+    """Checks a table and its lengths; the arguments that describe them to the native call."""
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise ValueError("block_table must be int32 [requests, blocks]")
     n, width = block_table.shape
-    _need(context_lens.dim() == 1 and context_lens.dtype == torch.int32 and context_lens.shape[0] == n,
-          "context_lens must be int32 [requests]")
-    _need(block_table.device == device and context_lens.device == device, "all tensors must be on one CUDA device")
-    _need(n <= MAX_REQUESTS, f"at most {MAX_REQUESTS} requests")
-    _need(block <= MAX_BLOCK, f"at most {MAX_BLOCK} tokens a block")
-    _need(width * block <= 2**31 - 2 * MAX_BLOCK, "block_table is too wide: a request has at most 2**31 tokens")
-    _need(n * width * block < 2**35, "block_table is too large: at most 2**35 tokens in all")
-    _need(width <= 1 or block_table.stride(1) == 1, "block_table's rows must be contiguous")
-    _need(n <= 1 or context_lens.stride(0) == 1, "context_lens must be contiguous")
-    return native().KvRequests(block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), n, width)
+    if n > MAX_REQUESTS:
+        raise ValueError(f"at most {MAX_REQUESTS} requests")
+    if context_lens.dtype != torch.int32 or context_lens.shape != (n,):
+        raise ValueError("context_lens must be int32 [requests]")
+    if block_table.get_device() != device or context_lens.get_device() != device:
+        raise ValueError("all tensors must be on one CUDA device")
+    row, col = block_table.stride()
+    if block > MAX_BLOCK:
+        raise ValueError(f"at most {MAX_BLOCK} tokens a block")
+    if width * block > 2**31 - 2 * MAX_BLOCK:
+        raise ValueError("block_table is too wide: a request has at most 2**31 tokens")
+    if n * width * block >= 2**35:
+        raise ValueError("block_table is too large: at most 2**35 tokens in all")
+    if col != 1 and width > 1:
+        raise ValueError("block_table's rows must be contiguous")
+    if n > 1 and not context_lens.is_contiguous():
+        raise ValueError("context_lens must be contiguous")
+    return block_table.data_ptr(), row, context_lens.data_ptr(), n, width
 
 
-def _cache(kv):
-    """Checked ``PagedKv`` of a layer's cache."""
-    _need(kv.dim() == 5 and kv.shape[0] == 2, "kv must be [2, pages, block, kv_heads, dim]")
+def _cache(torch, kv):
+    """Checks a layer's cache; the arguments that describe it to the native call."""
+    if kv.dim() != 5 or kv.shape[0] != 2:
+        raise ValueError("kv must be [2, pages, block, kv_heads, dim]")
+    kind = _kv_type(kv.dtype, torch)
     _, pages, block, heads, dim = kv.shape
-    kind = _kv_type(kv.dtype)
-    _need(heads >= 1 and block >= 1 and dim % 8 == 0 and 8 <= dim <= MAX_DIM,
-          f"kv's dim must be a multiple of 8 from 8 to {MAX_DIM}, and it must have heads and tokens")
-    _need(pages < 2**31, "too many pages")
     lane, page, token, head, last = kv.stride()
-    _need(last == 1, "kv's last dimension must be contiguous")
-    _need((kv.data_ptr() | 2 * lane | 2 * page | 2 * token | 2 * head) % 16 == 0,
-          "kv's address and strides must be multiples of 16 bytes")
-    return native().PagedKv(kv.data_ptr(), lane, page, token, head, pages, block, heads, dim, kind)
+    at = kv.data_ptr()
+    if dim % 8 or not 8 <= dim <= MAX_DIM or heads < 1 or block < 1:
+        raise ValueError(f"kv's dim must be a multiple of 8 from 8 to {MAX_DIM}, and it must have heads and tokens")
+    if pages >= 2**31:
+        raise ValueError("too many pages")
+    if last != 1:
+        raise ValueError("kv's last dimension must be contiguous")
+    if at % 16 or (lane | page | token | head) % 8:
+        raise ValueError("kv's address and strides must be multiples of 16 bytes")
+    return at, lane, page, token, head, pages, block, heads, dim, kind
 
 
-def _query(q, device, dtype, dim: int, kv_heads: int, requests: int):
-    _need(q.dim() == 3 and q.dtype == dtype and q.device == device,
-          "q must be [requests, heads, dim] in the cache's type and on its device")
-    _need(q.shape[0] == requests, "q and block_table must have as many requests")
-    _need(q.shape[2] == dim and q.shape[1] >= 1 and q.shape[1] % kv_heads == 0,
-          "q's dim must be the cache's, and its heads a multiple of the cache's")
-    # pairs are loaded at once: a view that splits them is copied
-    if q.stride(2) != 1 or (q.data_ptr() | 2 * q.stride(0) | 2 * q.stride(1)) % 4:
-        q = q.clone(memory_format=_torch().contiguous_format)
-    return q
+def _query(torch, q, device: int, dtype, dim: int, kv_heads: int, requests: int):
+    """Checks the queries; pairs are loaded at once, so a view that splits them is copied."""
+    if q.dim() != 3 or q.dtype != dtype or q.get_device() != device:
+        raise ValueError("q must be [requests, heads, dim] in the cache's type and on its device")
+    n, heads, d = q.shape
+    if n != requests:
+        raise ValueError("q and block_table must have as many requests")
+    if d != dim or heads < 1 or heads % kv_heads:
+        raise ValueError("q's dim must be the cache's, and its heads a multiple of the cache's")
+    row, head, last = q.stride()
+    at = q.data_ptr()
+    if last != 1 or at % 4 or (row | head) % 2:
+        q = q.clone(memory_format=torch.contiguous_format)
+        at, row, head = q.data_ptr(), heads * dim, dim
+    return q, (at, row, head, heads)
 
 
 def _overlap(a, b) -> bool:
@@ -151,41 +166,49 @@ def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=N
     that is a multiple of 16 and takes no ``blocks``.
     """
     torch = _torch()
-    cache = _cache(kv)
-    dev, dim, kv_heads, block = kv.device, kv.shape[4], kv.shape[3], kv.shape[2]
-    req = _requests(block_table, context_lens, dev, block)
-    n, width = block_table.shape
-    q = _query(q, dev, kv.dtype, dim, kv_heads, n)
-    _no_grad(q, kv)
-    heads = q.shape[1]
+    cache = _cache(torch, kv)
+    pages, block, kv_heads, dim = cache[5:9]
+    dev, index = kv.device, kv.get_device()
+    req = _requests(torch, block_table, context_lens, index, block)
+    n, width = req[3:]
+    q, query = _query(torch, q, index, kv.dtype, dim, kv_heads, n)
+    heads = query[3]
+    listed = weights = (0, 0)
     if blocks is not None:
-        _need(blocks.dtype == torch.int32 and blocks.device == dev and blocks.dim() == 3 and blocks.is_contiguous()
-              and blocks.shape[:2] == (n, kv_heads), "blocks must be contiguous int32 [requests, kv_heads, n]")
+        if (blocks.dtype != torch.int32 or blocks.get_device() != index or blocks.dim() != 3 or not blocks.is_contiguous()
+                or blocks.shape[:2] != (n, kv_heads)):
+            raise ValueError("blocks must be contiguous int32 [requests, kv_heads, n]")
+        listed = blocks.data_ptr(), blocks.shape[2]
     if mass is not None:
-        _need(blocks is None, "mass is gathered over all blocks: it takes no blocks=")
-        _need(block % 16 == 0, "mass needs a block size that is a multiple of 16")
-        _need(mass.dtype == torch.float32 and mass.device == dev and mass.shape == block_table.shape,
-              "mass must be fp32 in block_table's shape")
-        _need((width <= 1 or mass.stride(1) == 1) and (n <= 1 or mass.stride(0) >= width),
-              "mass must have contiguous rows of their own")
+        if blocks is not None:
+            raise ValueError("mass is gathered over all blocks: it takes no blocks=")
+        if block % 16:
+            raise ValueError("mass needs a block size that is a multiple of 16")
+        if mass.dtype != torch.float32 or mass.get_device() != index or mass.shape != block_table.shape:
+            raise ValueError("mass must be fp32 in block_table's shape")
+        row, col = mass.stride()
+        if (width > 1 and col != 1) or (n > 1 and row < width):
+            raise ValueError("mass must have contiguous rows of their own")
+        weights = mass.data_ptr(), row
     if out is not None:
-        _need(out.dtype == q.dtype and out.device == dev and out.shape == q.shape and out.is_contiguous()
-              and out.data_ptr() % 4 == 0, "out must be contiguous, like q, on a 4-byte boundary")
-        _need(not _overlap(out, q) and not _overlap(out, kv), "out must not overlap q or kv")
-    _cuda(dev)
+        if (out.dtype != q.dtype or out.get_device() != index or out.shape != q.shape or not out.is_contiguous()
+                or out.data_ptr() % 4):
+            raise ValueError("out must be contiguous, like q, on a 4-byte boundary")
+        if _overlap(out, q) or _overlap(out, kv):
+            raise ValueError("out must not overlap q or kv")
+    stream = _runs(torch, kv, q)
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-    lse = torch.empty((n, heads), dtype=torch.float32, device=dev)
-    call = native().KvAttention(cache, req, q.data_ptr(), q.stride(0), q.stride(1), heads,
-                                dim ** -0.5 if scale is None else float(scale),
-                                0 if blocks is None else blocks.data_ptr(), 0 if blocks is None else blocks.shape[2],
-                                0 if mass is None else mass.data_ptr(), 0 if mass is None else mass.stride(0))
-    if blocks is not None and blocks.shape[2] == 0:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+    lse = q.new_empty((n, heads), dtype=torch.float32)
+    if blocks is not None and listed[1] == 0:
         out.zero_()
         lse.fill_(float("-inf"))
     else:
-        work = torch.empty(call.work_bytes(dev.index), dtype=torch.uint8, device=dev)
-        call.run(out.data_ptr(), lse.data_ptr(), work.data_ptr(), dev.index, torch.cuda.current_stream(dev).cuda_stream)
+        C = native()
+        work = torch.empty(C.paged_kv_attention_work(n, width, block, heads, kv_heads, dim, mass is not None, index),
+                           dtype=torch.uint8, device=dev)
+        C.paged_kv_attention(*cache, *req, *query, dim ** -0.5 if scale is None else float(scale), *listed, *weights,
+                             out.data_ptr(), lse.data_ptr(), work.data_ptr(), index, stream)
     return (out, lse) if return_lse else out
 
 
@@ -198,18 +221,18 @@ def paged_kv_bounds(kv, block_table, context_lens, bounds, *, new_tokens=None):
     share has to be filled alike in both.  Returns ``bounds``.
     """
     torch = _torch()
-    cache = _cache(kv)
-    req = _requests(block_table, context_lens, kv.device, kv.shape[2])
-    _, pages, _, heads, dim = kv.shape
-    _no_grad(kv, bounds)
-    _need(bounds.dtype == kv.dtype and bounds.device == kv.device and bounds.shape == (pages, heads, 2, dim)
-          and bounds.is_contiguous() and bounds.data_ptr() % 16 == 0,
-          "bounds must be contiguous [pages, kv_heads, 2, dim] in the cache's type, on a 16-byte boundary")
-    _need(not _overlap(bounds, kv), "bounds must not overlap kv")
+    cache = _cache(torch, kv)
+    pages, block, heads, dim = cache[5:9]
+    index = kv.get_device()
+    req = _requests(torch, block_table, context_lens, index, block)
+    if (bounds.dtype != kv.dtype or bounds.get_device() != index or bounds.shape != (pages, heads, 2, dim)
+            or not bounds.is_contiguous() or bounds.data_ptr() % 16):
+        raise ValueError("bounds must be contiguous [pages, kv_heads, 2, dim] in the cache's type, on a 16-byte boundary")
+    if _overlap(bounds, kv):
+        raise ValueError("bounds must not overlap kv")
     since = -1 if new_tokens is None else _int(new_tokens, "new_tokens", 0)
-    _cuda(kv.device)
-    native().paged_kv_bounds(cache, req, since, bounds.data_ptr(), kv.device.index,
-                             torch.cuda.current_stream(kv.device).cuda_stream)
+    stream = _runs(torch, kv, bounds)
+    native().paged_kv_bounds(*cache, *req, since, bounds.data_ptr(), index, stream)
     return bounds
 
 
@@ -227,26 +250,25 @@ def paged_kv_select(q, bounds, block_table, context_lens, keep, *, block_size, s
     are no row of ``bounds`` are not taken.
     """
     torch = _torch()
-    _need(bounds.dim() == 4 and bounds.shape[2] == 2 and bounds.is_contiguous() and bounds.data_ptr() % 16 == 0,
-          "bounds must be contiguous [pages, kv_heads, 2, dim] on a 16-byte boundary")
-    dev = bounds.device
+    if bounds.dim() != 4 or bounds.shape[2] != 2 or not bounds.is_contiguous() or bounds.data_ptr() % 16:
+        raise ValueError("bounds must be contiguous [pages, kv_heads, 2, dim] on a 16-byte boundary")
     pages, kv_heads, _, dim = bounds.shape
-    kind = _kv_type(bounds.dtype)
-    _need(kv_heads >= 1 and dim % 8 == 0 and 8 <= dim <= MAX_DIM and pages < 2**31,
-          f"bounds' dim must be a multiple of 8 from 8 to {MAX_DIM}")
+    index = bounds.get_device()
+    kind = _kv_type(bounds.dtype, torch)
+    if kv_heads < 1 or dim % 8 or not 8 <= dim <= MAX_DIM or pages >= 2**31:
+        raise ValueError(f"bounds' dim must be a multiple of 8 from 8 to {MAX_DIM}")
     block = _int(block_size, "block_size", 1)
-    req = _requests(block_table, context_lens, dev, block)
-    n, width = block_table.shape
-    q = _query(q, dev, bounds.dtype, dim, kv_heads, n)
-    _no_grad(q, bounds)
+    req = _requests(torch, block_table, context_lens, index, block)
+    n, width = req[3:]
+    q, query = _query(torch, q, index, bounds.dtype, dim, kv_heads, n)
     keep, sink, recent = _int(keep, "keep", 1), _int(sink, "sink", 0), _int(recent, "recent", 0)
-    _need(sink + recent <= keep, "keep must be at least sink + recent")
-    _cuda(dev)
-    out = torch.empty((n, kv_heads, keep), dtype=torch.int32, device=dev)
-    scores = torch.empty((n, kv_heads, width), dtype=torch.float32, device=dev)
-    native().paged_kv_select(req, q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], bounds.data_ptr(), pages, block,
-                             kv_heads, dim, kind, keep, sink, recent, scores.data_ptr(), out.data_ptr(), dev.index,
-                             torch.cuda.current_stream(dev).cuda_stream)
+    if sink + recent > keep:
+        raise ValueError("keep must be at least sink + recent")
+    stream = _runs(torch, bounds, q)
+    out = block_table.new_empty((n, kv_heads, keep))
+    scores = torch.empty(n * kv_heads * width, dtype=torch.float32, device=bounds.device)
+    native().paged_kv_select(*req, *query, bounds.data_ptr(), pages, block, kv_heads, dim, kind, keep, sink, recent,
+                             scores.data_ptr(), out.data_ptr(), index, stream)
     return out
 
 
@@ -270,23 +292,26 @@ def paged_kv_evict(mass, block_table, context_lens, budget, *, block_size, sink=
     dropped and not listed.  The inputs are left as they were.
     """
     torch = _torch()
-    _need(mass.dtype == torch.float32 and mass.shape == block_table.shape, "mass must be fp32 in block_table's shape")
-    dev = mass.device
+    if mass.dtype != torch.float32 or mass.shape != block_table.shape:
+        raise ValueError("mass must be fp32 in block_table's shape")
+    index = mass.get_device()
     block = _int(block_size, "block_size", 1)
-    req = _requests(block_table, context_lens, dev, block)
-    n, width = mass.shape
-    _need(width <= 1 or mass.stride(1) == 1, "mass' rows must be contiguous")
+    req = _requests(torch, block_table, context_lens, index, block)
+    n, width = req[3:]
+    row, col = mass.stride()
+    if width > 1 and col != 1:
+        raise ValueError("mass' rows must be contiguous")
     budget, sink, recent = _int(budget, "budget", 1), _int(sink, "sink", 0), _int(recent, "recent", 1)
-    _need(sink + recent <= budget, "budget must be at least sink + recent")
-    _cuda(dev)
-    e = KVEviction(*(torch.empty(s, dtype=t, device=dev) for s, t in (
-        ((n, width), torch.int32), ((n,), torch.int32), ((n, width), torch.float32), ((n, width), torch.int32),
-        ((n, width), torch.int32), ((n,), torch.int32))))
-    native().paged_kv_evict(req, mass.data_ptr(), mass.stride(0), block, budget, sink, recent,
-                            e.block_table.data_ptr(), e.context_lens.data_ptr(), e.mass.data_ptr(),
-                            e.evicted_blocks.data_ptr(), e.evicted_index.data_ptr(), e.evicted_count.data_ptr(),
-                            dev.index, torch.cuda.current_stream(dev).cuda_stream)
-    return e
+    if sink + recent > budget:
+        raise ValueError("budget must be at least sink + recent")
+    stream = _runs(torch, mass)
+    # two allocations: an allocation costs as much host time as the launch
+    table, pages, places, kept = block_table.new_empty((4, n, width)).unbind(0)
+    lens, count = context_lens.new_empty((2, n)).unbind(0)
+    kept = kept.view(torch.float32)
+    native().paged_kv_evict(*req, mass.data_ptr(), row, block, budget, sink, recent, table.data_ptr(), lens.data_ptr(),
+                            kept.data_ptr(), pages.data_ptr(), places.data_ptr(), count.data_ptr(), index, stream)
+    return KVEviction(table, lens, kept, pages, places, count)
 
 
 __all__ = ["KVEviction", "paged_kv_attention", "paged_kv_bounds", "paged_kv_evict", "paged_kv_select"]

@@ -136,6 +136,7 @@ def test_a_query_that_splits_pairs_is_copied(good):
     spread = torch.zeros(*q.shape, 2, dtype=q.dtype)[..., 0].copy_(q)
     rows = torch.zeros(2, 8, 65, dtype=q.dtype)[..., :64].copy_(q)
     for x in (odd, spread, rows):
-        got = _query(x, q.device, q.dtype, 64, 2, 2)
+        got, (at, row, head, heads) = _query(torch, x, -1, q.dtype, 64, 2, 2)
+        assert (at, row, head, heads) == (got.data_ptr(), 512, 64, 8)
         assert got.data_ptr() % 4 == 0 and got.is_contiguous() and torch.equal(got, q)
-    assert _query(q, q.device, q.dtype, 64, 2, 2) is q
+    assert _query(torch, q, -1, q.dtype, 64, 2, 2)[0] is q
