@@ -155,14 +155,17 @@ __device__ __forceinline__ uint32_t tiles_of(const KvAttention& a, int len) {
   return static_cast<uint32_t>((static_cast<long long>(slots_of(a, len)) * a.kv.block + kTile - 1) / kTile);
 }
 
-// first[b] of every request and of their end, by the whole CTA.
-__device__ __forceinline__ void first_tiles(const KvAttention& a, uint32_t* first, uint32_t* scratch) {
+// first[b] of every request and of their end, and the requests' lengths, by the
+// whole CTA.
+__device__ __forceinline__ void first_tiles(const KvAttention& a, uint32_t* first, int* lens, uint32_t* scratch) {
   const int n = a.req.requests, per = (n + blockDim.x - 1) / blockDim.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int b0 = min(n, static_cast<int>(threadIdx.x) * per), b1 = min(n, b0 + per);
   uint32_t mine = 0;
   for (int b = b0; b < b1; ++b) {
+    const int len = length_of(a, b);
+    lens[b] = len;
     first[b] = mine;
-    mine += tiles_of(a, length_of(a, b));
+    mine += tiles_of(a, len);
   }
   uint32_t upto = mine;
 #pragma unroll
@@ -202,13 +205,14 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
   __shared__ uint32_t scratch[S::kWarps];
   __shared__ uint32_t valid_of[S::kWarps][S::kStages];
   uint32_t* first = reinterpret_cast<uint32_t*>(smem + S::kRingBytes);
+  int* lens = reinterpret_cast<int*>(first + a.req.requests + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int D = a.kv.dim, bs = a.kv.block, G = a.q.heads / a.kv.kv_heads, n = a.req.requests;
   launch_dependents();
   if (D < DP)  // what the copies leave of a row stays zero
     for (int i = threadIdx.x; i < S::kRingBytes / 16; i += blockDim.x)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-  first_tiles(a, first, scratch);
+  first_tiles(a, first, lens, scratch);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= n; i += blockDim.x) w.first[i] = first[i];
   const KvPlan plan = KvPlan::make(first[n], w.most_ranges, kLeastTiles);
@@ -227,36 +231,74 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     const uint32_t lo = static_cast<uint32_t>(plan.begin(r)), hi = static_cast<uint32_t>(plan.begin(r + 1));
     const T* cache = static_cast<const T*>(a.kv.base) + g * a.kv.head_stride;
 
-    // ---- the tiles' places and copies --------------------------------------------
-    uint32_t next = lo;  // the tile that is looked up next
-    int lb = request_of(first, n, lo), llen = length_of(a, lb), lslots = slots_of(a, llen);
-    long long row_at = 0;  // of lanes 0-15: where the row of the tile looked up last begins
-    bool row_ok = false;
-    auto look_up = [&]() {
-      row_ok = false;
-      if (next < hi) {
-        while (next >= first[lb + 1]) {
-          ++lb;
-          llen = length_of(a, lb);
-          lslots = slots_of(a, llen);
+    // ---- the heads' rows of a request ------------------------------------------------
+    float o[DP / 8][4], m[2], l[2];
+    uint32_t q[DP / 16][4];
+    int b = request_of(first, n, lo);
+    uint32_t end = 0;  // of request b's tiles
+    auto begin_request = [&]() {
+      end = first[b + 1];
+      const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+          q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
+                        ? 0u
+                        : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
         }
-        const uint32_t t = (next - first[lb]) * kTile + (lane & 15);
-        const int slot = static_cast<int>(t / static_cast<uint32_t>(bs)), off = static_cast<int>(t - slot * static_cast<uint32_t>(bs));
-        int block = slot;
-        bool ok = slot < lslots;
-        if (a.blocks != nullptr) {
-          block = ok ? a.blocks[(static_cast<long long>(lb) * a.kv.kv_heads + g) * a.blocks_width + slot] : -1;
-          ok = block >= 0;
-        }
-        ok = ok && static_cast<long long>(block) * bs + off < llen;
-        const int page = ok ? a.req.table[lb * a.req.table_stride + block] : -1;
-        row_ok = page >= 0 && page < a.kv.pages;
-        row_at = row_ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
-      }
-      ++next;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
     };
+    begin_request();
+
+    // ---- the tiles' places and copies --------------------------------------------
+    // A window is 32 neighbouring blocks of a request, a lane each: their pages, and
+    // how many tokens of each count.  The next window is looked up while this one is
+    // used.
+    struct Window {
+      int b, slot;         // its request and first block
+      uint32_t from, end;  // the tiles that lie in it
+      int page, tokens;    // of this lane's block
+    };
+    auto look_up = [&](uint32_t tile, int request) {
+      Window v;
+      v.b = request;
+      v.from = v.end = tile;
+      v.slot = v.page = v.tokens = 0;
+      if (tile >= hi) return v;
+      while (first[v.b + 1] <= tile) ++v.b;
+      const int len = lens[v.b], blocks = (len + bs - 1) / bs;
+      v.slot = static_cast<int>((tile - first[v.b]) * kTile / static_cast<uint32_t>(bs));
+      int block = v.slot + lane;
+      if (a.blocks != nullptr)
+        block = block < min(blocks, a.blocks_width)
+                    ? a.blocks[(static_cast<long long>(v.b) * a.kv.kv_heads + g) * a.blocks_width + block]
+                    : -1;
+      v.page = -1;
+      if (block >= 0 && block < blocks) {
+        v.tokens = min(bs, len - block * bs);
+        v.page = a.req.table[v.b * a.req.table_stride + block];
+      }
+      const long long tiles = (v.slot + 32ll) * bs / kTile;  // whose blocks all lie in the window
+      v.end = static_cast<uint32_t>(min(first[v.b] + tiles, static_cast<long long>(min(first[v.b + 1], hi))));
+      return v;
+    };
+    Window now = look_up(lo, b), next = look_up(now.end, now.b);
     constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
-    auto copy = [&](int stage) {
+    auto copy = [&](int stage, uint32_t tile) {
+      if (tile >= now.end) {
+        now = next;
+        next = look_up(now.end, now.b);
+      }
+      const uint32_t t = (tile - first[now.b]) * kTile + (lane & 15);
+      const int slot = static_cast<int>(t / static_cast<uint32_t>(bs)), off = static_cast<int>(t - slot * static_cast<uint32_t>(bs));
+      const int page = __shfl_sync(0xffffffffu, now.page, slot - now.slot);
+      const bool row_ok = off < __shfl_sync(0xffffffffu, now.tokens, slot - now.slot) && page >= 0 && page < a.kv.pages;
+      const long long row_at = row_ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
       const uint32_t ok = __ballot_sync(0xffffffffu, row_ok) & 0xffffu;
       if (lane == 0) valid_of[warp][stage] = ok;
       const uint32_t to = ring + stage * S::kStageBytes;
@@ -273,48 +315,27 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
         }
       }
     };
-    look_up();
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; ++i) {
-      if (lo + i < hi) copy(i);
+      if (lo + i < hi) copy(i, lo + i);
       cp_commit();
-      look_up();
     }
 
     // ---- the products ----------------------------------------------------------------
-    float o[DP / 8][4], m[2], l[2];
-    uint32_t q[DP / 16][4];
     const float to_base2 = a.scale * kLog2e;
-    int b = -1;
-    uint32_t end = 0;  // of request b's tiles
     int stage = 0;
     for (uint32_t tile = lo; tile < hi; ++tile) {
-      if (b < 0 || tile >= end) {  // a new request: its heads' rows
-        b = b < 0 ? request_of(first, n, tile) : b + 1;
-        while (first[b + 1] <= tile) ++b;
-        end = first[b + 1];
-        const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
-            q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
-                          ? 0u
-                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
-          }
-#pragma unroll
-        for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
+      if (tile >= end) {
+        do ++b;
+        while (first[b + 1] <= tile);
+        begin_request();
       }
       cp_wait<S::kStages - 2>();
       __syncwarp();
       {  // the stage that the last step emptied
         const int into = stage == 0 ? S::kStages - 1 : stage - 1;
-        if (tile + S::kStages - 1 < hi) copy(into);
+        if (tile + S::kStages - 1 < hi) copy(into, tile + S::kStages - 1);
         cp_commit();
-        look_up();
       }
       const uint32_t ok = valid_of[warp][stage];
       const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + kTile * DP * 2;
@@ -598,15 +619,15 @@ cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaSt
 
 template <typename T, int DP>
 cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cudaStream_t stream) {
-  const int smem = Shape<DP>::kRingBytes + (a.req.requests + 1) * 4, threads = Shape<DP>::kWarps * 32;
+  const int smem = Shape<DP>::kRingBytes + (2 * a.req.requests + 1) * 4, threads = Shape<DP>::kWarps * 32;
   auto kernel = w.rows == 8 ? attention_kernel<T, DP, true> : attention_kernel<T, DP, false>;
-  static_assert(Shape<DP>::kRingBytes + (kMostRequests + 1) * 4 <= 230 * 1024, "more shared memory than an SM has");
+  static_assert(Shape<DP>::kRingBytes + (2 * kMostRequests + 1) * 4 <= 226 * 1024, "more shared memory than an SM has");
   static std::atomic<uint64_t> ready[2];  // devices that know the kernels' shared memory
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   cudaError_t rc = cudaSuccess;
   if (!(ready[w.rows == 8].load(std::memory_order_relaxed) & bit)) {
     rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              Shape<DP>::kRingBytes + (kMostRequests + 1) * 4);
+                              Shape<DP>::kRingBytes + (2 * kMostRequests + 1) * 4);
     if (rc != cudaSuccess) return rc;
     ready[w.rows == 8].fetch_or(bit, std::memory_order_relaxed);
   }
