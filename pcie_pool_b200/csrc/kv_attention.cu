@@ -54,6 +54,7 @@ struct Work {
   float* part_o;        // [2 ranges, groups, rows, dim]
   float2* part_ml;      // [2 ranges, groups, rows]: maximum (base 2) and sum
   uint32_t* first;      // [requests + 1]
+  int* begins;          // [ranges]: the request of a range's first tile
   float* z;             // [requests, max_tiles, heads]: log2 of a tile's sum, or null
   int max_tiles;        // of a request
   int most_ranges;
@@ -215,6 +216,12 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
   first_tiles(a, first, lens, scratch);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= n; i += blockDim.x) w.first[i] = first[i];
+  for (int b = blockIdx.x; b < n; b += gridDim.x)  // requests without tokens
+    if (first[b] == first[b + 1]) {
+      for (int i = 2 * threadIdx.x; i < a.q.heads * D; i += 2 * blockDim.x)
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + static_cast<long long>(b) * a.q.heads * D + i) = 0u;
+      for (int i = threadIdx.x; i < a.q.heads; i += blockDim.x) a.lse[static_cast<long long>(b) * a.q.heads + i] = -INFINITY;
+    }
   const KvPlan plan = KvPlan::make(first[n], w.most_ranges, kLeastTiles);
   if (plan.tiles == 0) return;
   const long long units = static_cast<long long>(plan.ranges) * w.groups;
@@ -235,6 +242,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     float o[DP / 8][4], m[2], l[2];
     uint32_t q[DP / 16][4];
     int b = request_of(first, n, lo);
+    if (group == 0 && lane == 0) w.begins[r] = b;
     uint32_t end = 0;  // of request b's tiles
     auto begin_request = [&]() {
       end = first[b + 1];
@@ -461,93 +469,107 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
   }
 }
 
-// Adds up what the ranges left of a request that was cut: a CTA for each query
-// head, its warps take four parts at a time.  Requests without tokens get zeros.
-constexpr int kJoinWarps = 8, kJoinParts = 4;
+// Adds up what the ranges left of a request that was cut.  There are no more cuts
+// than ranges: with few requests a CTA goes by a request, with many by a range's
+// begin, and is the one to work if that is the first cut of its request.  Its eight
+// warps share `heads_each` query heads; a warp takes eight parts at a time, whose
+// loads are in flight together.
+constexpr int kJoinWarps = 8, kJoinParts = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ KvAttention a,
-                                                                         const __grid_constant__ Work w) {
-  __shared__ __align__(16) float sum_o[kJoinWarps][256];
+template <typename T, int DP>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    attention_join_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w, int heads_each, bool by_cut) {
+  constexpr int kVecs = DP / 64;  // pairs of a lane
+  __shared__ __align__(16) float sum_o[kJoinWarps][DP];
   __shared__ float sum_m[kJoinWarps], sum_l[kJoinWarps];
-  const int b = blockIdx.x / a.q.heads, h = blockIdx.x % a.q.heads, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps_each = kJoinWarps / heads_each;
+  const int h = blockIdx.x * heads_each + warp / warps_each, mine = warp % warps_each;
   const int D = a.kv.dim, G = a.q.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
-  const int group = h / G * per_head + h % G / kRowGroup, row = h % G % kRowGroup;
-  T* out = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.q.heads + h) * D;
-  float* lse = a.lse + static_cast<long long>(b) * a.q.heads + h;
   wait_for_parent();
-  const uint32_t f0 = w.first[b], f1 = w.first[b + 1], tiles = w.first[a.req.requests];
-  if (f0 == f1) {
-    for (int d = 2 * threadIdx.x; d < D; d += 2 * blockDim.x) *reinterpret_cast<uint32_t*>(out + d) = 0u;
-    if (threadIdx.x == 0) *lse = -INFINITY;
-    return;
-  }
+  const uint32_t tiles = w.first[a.req.requests];
+  if (tiles == 0) return;
   const KvPlan plan = KvPlan::make(tiles, w.most_ranges, kLeastTiles);
+  int b = blockIdx.y;
+  if (by_cut) {
+    if (b + 1 >= plan.ranges) return;
+    b = w.begins[b + 1];
+  }
+  const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
+  if (f0 == f1) return;
   const int r0 = plan.of(f0), r1 = plan.of(f1 - 1);
-  if (r0 == r1) return;  // finished where it was computed
-  // the first part may lie in its range's second place, the others lie in the first
-  const long long base = static_cast<long long>(group) * w.rows + row, step = static_cast<long long>(w.groups) * w.rows;
-  const int slot0 = plan.slot(r0, f0);
-  float m = -INFINITY, l = 0.f, o[8] = {};
-  for (int r = r0 + warp * kJoinParts; r <= r1; r += kJoinWarps * kJoinParts) {
-    float2 ml[kJoinParts];
-    float4 v[kJoinParts][2];
+  if (r0 == r1 || (by_cut && r0 != static_cast<int>(blockIdx.y))) return;  // finished where it was computed
+  float m = -INFINITY, l = 0.f;
+  float2 o[kVecs];
 #pragma unroll
-    for (int k = 0; k < kJoinParts; ++k) {
-      const long long at = base + step * (r + k == r0 ? slot0 : 2 * (r + k));
-      ml[k] = make_float2(-INFINITY, 0.f);
-      v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r + k <= r1) {
-        ml[k] = w.part_ml[at];
+  for (int i = 0; i < kVecs; ++i) o[i] = make_float2(0.f, 0.f);
+  if (h < a.q.heads) {
+    // the first part may lie in its range's second place, the others lie in the first
+    const long long base = static_cast<long long>(h / G * per_head + h % G / kRowGroup) * w.rows + h % G % kRowGroup;
+    const long long step = static_cast<long long>(w.groups) * w.rows;
+    const int slot0 = plan.slot(r0, f0);
+    for (int r = r0 + mine * kJoinParts; r <= r1; r += warps_each * kJoinParts) {
+      float2 ml[kJoinParts], v[kJoinParts][kVecs];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i * 128 + lane * 4 < D) v[k][i] = *reinterpret_cast<const float4*>(w.part_o + at * D + i * 128 + lane * 4);
+      for (int k = 0; k < kJoinParts; ++k) {
+        const long long at = base + step * (r + k == r0 ? slot0 : 2 * (r + k));
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (r + k <= r1) ml[k] = w.part_ml[at];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          v[k][i] = make_float2(0.f, 0.f);
+          if (r + k <= r1 && i * 64 + lane * 2 < D) v[k][i] = *reinterpret_cast<const float2*>(w.part_o + at * D + i * 64 + lane * 2);
+        }
+      }
+      float now = m;
+#pragma unroll
+      for (int k = 0; k < kJoinParts; ++k) now = fmaxf(now, ml[k].x);
+      const float ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref);
+      m = now;
+      l *= c;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) o[i].x *= c, o[i].y *= c;
+#pragma unroll
+      for (int k = 0; k < kJoinParts; ++k) {
+        const float p = ex2(ml[k].x - ref);
+        l += ml[k].y * p;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) o[i].x += v[k][i].x * p, o[i].y += v[k][i].y * p;
       }
     }
-    float now = m;
+  }
+  if (warps_each > 1) {
+    if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
 #pragma unroll
-    for (int k = 0; k < kJoinParts; ++k) now = fmaxf(now, ml[k].x);
-    const float ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref);
-    m = now;
-    l *= c;
+    for (int i = 0; i < kVecs; ++i) *reinterpret_cast<float2*>(&sum_o[warp][i * 64 + lane * 2]) = o[i];
+    __syncthreads();
+    if (mine != 0) return;
+    float top = -INFINITY;
+    for (int i = 0; i < warps_each; ++i) top = fmaxf(top, sum_m[warp + i]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    m = top;
+    l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] *= c;
+    for (int i = 0; i < kVecs; ++i) o[i] = make_float2(0.f, 0.f);
+    for (int k = 0; k < warps_each; ++k) {
+      const float p = ex2(sum_m[warp + k] - ref);
+      l += p * sum_l[warp + k];
 #pragma unroll
-    for (int k = 0; k < kJoinParts; ++k) {
-      const float p = ex2(ml[k].x - ref);
-      l += ml[k].y * p;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        o[4 * i] += v[k][i].x * p;
-        o[4 * i + 1] += v[k][i].y * p;
-        o[4 * i + 2] += v[k][i].z * p;
-        o[4 * i + 3] += v[k][i].w * p;
+      for (int i = 0; i < kVecs; ++i) {
+        const float2 v = *reinterpret_cast<const float2*>(&sum_o[warp + k][i * 64 + lane * 2]);
+        o[i].x += v.x * p;
+        o[i].y += v.y * p;
       }
     }
   }
-  if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
+  if (h >= a.q.heads) return;
+  const long long row = static_cast<long long>(b) * a.q.heads + h;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    *reinterpret_cast<float4*>(&sum_o[warp][i * 128 + lane * 4]) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-  __syncthreads();
-  float top = -INFINITY, total = 0.f, by[kJoinWarps];
-#pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, sum_m[i]);
-#pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) {
-    by[i] = ex2(sum_m[i] - (top == -INFINITY ? 0.f : top));
-    total += by[i] * sum_l[i];
+  for (int i = 0; i < kVecs; ++i) {
+    const int d = i * 64 + lane * 2;
+    if (d < D)
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + row * D + d) = l == 0.f ? 0u : Type<T>::pack(o[i].x / l, o[i].y / l);
   }
-  for (int d = 2 * threadIdx.x; d < D; d += 2 * blockDim.x) {
-    float u = 0.f, v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) {
-      u += by[i] * sum_o[i][d];
-      v += by[i] * sum_o[i][d + 1];
-    }
-    *reinterpret_cast<uint32_t*>(out + d) = total == 0.f ? 0u : Type<T>::pack(u / total, v / total);
-  }
-  if (threadIdx.x == 0) *lse = total == 0.f ? -INFINITY : (top + lg2(total)) * kLn2;
+  if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
 // A warp for each block: the tiles' sums of every head, weighed by the head's total.
@@ -590,6 +612,8 @@ uint64_t lay_out(int requests, int width, int block, int heads, int kv_heads, in
   at += up(parts * 8);
   w.first = reinterpret_cast<uint32_t*>(p + at);
   at += up((requests + 1ull) * 4);
+  w.begins = reinterpret_cast<int*>(p + at);
+  at += up(w.most_ranges * 4ull);
   w.z = mass ? reinterpret_cast<float*>(p + at) : nullptr;
   if (mass) at += up(uint64_t(requests) * w.max_tiles * heads * 4);
   return at;
@@ -602,9 +626,8 @@ cudaError_t sm_count(int* sms, int* device) {
 
 // A kernel that may be resident before the one ahead of it in the stream is done
 // (it waits for it itself).
-template <typename... Args>
-cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t stream, const KvAttention& a,
-                         const Work& w) {
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(threads);
@@ -614,7 +637,7 @@ cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaSt
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, a, w);
+  return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 template <typename T, int DP>
@@ -634,7 +657,14 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
   kernel<<<sms, threads, smem, stream>>>(a, w);
   rc = cudaGetLastError();
   if (rc != cudaSuccess) return rc;
-  return launch_after(attention_join_kernel<T>, dim3(a.req.requests * a.q.heads), kJoinWarps * 32, stream, a, w);
+  // as many warps for a head as leave four CTAs to an SM
+  const bool by_cut = a.req.requests >= w.most_ranges;
+  const int items = by_cut ? w.most_ranges - 1 : a.req.requests;
+  if (items == 0) return cudaSuccess;
+  int heads_each = 1;
+  while (heads_each < kJoinWarps && static_cast<int64_t>(items) * ((a.q.heads + heads_each - 1) / heads_each) > 4 * sms) heads_each *= 2;
+  return launch_after(attention_join_kernel<T, DP>, dim3((a.q.heads + heads_each - 1) / heads_each, items), kJoinWarps * 32,
+                      stream, a, w, heads_each, by_cut);
 }
 
 template <typename T>

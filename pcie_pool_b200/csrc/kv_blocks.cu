@@ -564,6 +564,8 @@ void for_width(int width, Launch launch) {
     launch(integral_constant<int, 128>(), integral_constant<int, 8>());
   else if (width <= 4096)
     launch(integral_constant<int, 256>(), integral_constant<int, 16>());
+  else if (width <= 8192)
+    launch(integral_constant<int, 512>(), integral_constant<int, 16>());
   else
     launch(integral_constant<int, 512>(), integral_constant<int, 32>());
 }
