@@ -48,6 +48,8 @@ struct Shape {
   static constexpr int kStages = DP == 64 ? 6 : 3;
   static constexpr int kStageBytes = 2 * kTile * DP * 2;  // K, then V
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  // of a thread: a quarter of the SM's registers is left for a CTA of the join
+  static constexpr int kRegisters = DP == 256 ? 255 : 192;
 };
 
 struct Work {
@@ -199,7 +201,7 @@ __device__ __forceinline__ int request_of(const uint32_t* first, int n, uint32_t
 // DP: dim padded to 64, 128 or 256.  PACKED: at most eight heads share a key head,
 // rows 8 to 15 carry the weights' remainders.
 template <typename T, int DP, bool PACKED>
-__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
+__global__ void __maxnreg__(Shape<DP>::kRegisters)
     attention_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w) {
   using S = Shape<DP>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -238,45 +240,27 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
     const uint32_t lo = static_cast<uint32_t>(plan.begin(r)), hi = static_cast<uint32_t>(plan.begin(r + 1));
     const T* cache = static_cast<const T*>(a.kv.base) + g * a.kv.head_stride;
 
-    // ---- the heads' rows of a request ------------------------------------------------
     float o[DP / 8][4], m[2], l[2];
     uint32_t q[DP / 16][4];
+    const float to_base2 = a.scale * kLog2e;
     int b = request_of(first, n, lo);
     if (group == 0 && lane == 0) w.begins[r] = b;
     uint32_t end = 0;  // of request b's tiles
-    auto begin_request = [&]() {
-      end = first[b + 1];
-      const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
-          q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
-                        ? 0u
-                        : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
-        }
-#pragma unroll
-      for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
-    };
-    begin_request();
 
-    // ---- the tiles' places and copies --------------------------------------------
     // A window is 32 neighbouring blocks of a request, a lane each: their pages, and
     // how many tokens of each count.  The next window is looked up while this one is
     // used.
     struct Window {
-      int b, slot;         // its request and first block
-      uint32_t from, end;  // the tiles that lie in it
-      int page, tokens;    // of this lane's block
+      int b, slot;   // its request and first block
+      uint32_t end;  // of the tiles that lie in it
+      int page, tokens;  // of this lane's block
     };
     auto look_up = [&](uint32_t tile, int request) {
       Window v;
       v.b = request;
-      v.from = v.end = tile;
-      v.slot = v.page = v.tokens = 0;
+      v.end = tile;
+      v.slot = v.tokens = 0;
+      v.page = -1;
       if (tile >= hi) return v;
       while (first[v.b + 1] <= tile) ++v.b;
       const int len = lens[v.b], blocks = (len + bs - 1) / bs;
@@ -286,7 +270,6 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
         block = block < min(blocks, a.blocks_width)
                     ? a.blocks[(static_cast<long long>(v.b) * a.kv.kv_heads + g) * a.blocks_width + block]
                     : -1;
-      v.page = -1;
       if (block >= 0 && block < blocks) {
         v.tokens = min(bs, len - block * bs);
         v.page = a.req.table[v.b * a.req.table_stride + block];
@@ -295,56 +278,68 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
       v.end = static_cast<uint32_t>(min(first[v.b] + tiles, static_cast<long long>(min(first[v.b + 1], hi))));
       return v;
     };
-    Window now = look_up(lo, b), next = look_up(now.end, now.b);
-    constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
-    auto copy = [&](int stage, uint32_t tile) {
-      if (tile >= now.end) {
-        now = next;
-        next = look_up(now.end, now.b);
-      }
-      const uint32_t t = (tile - first[now.b]) * kTile + (lane & 15);
-      const int slot = static_cast<int>(t / static_cast<uint32_t>(bs)), off = static_cast<int>(t - slot * static_cast<uint32_t>(bs));
-      const int page = __shfl_sync(0xffffffffu, now.page, slot - now.slot);
-      const bool row_ok = off < __shfl_sync(0xffffffffu, now.tokens, slot - now.slot) && page >= 0 && page < a.kv.pages;
-      const long long row_at = row_ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
-      const uint32_t ok = __ballot_sync(0xffffffffu, row_ok) & 0xffffu;
-      if (lane == 0) valid_of[warp][stage] = ok;
-      const uint32_t to = ring + stage * S::kStageBytes;
-#pragma unroll
-      for (int i = 0; i < kTile * kChunks / 32; ++i) {
-        const int row = (i * 32 + lane) / kChunks, chunk = (i * 32 + lane) % kChunks;
-        const long long at = __shfl_sync(0xffffffffu, row_at, row) + chunk * 8;
-        const uint32_t dst = to + row * DP * 2 + ((chunk ^ (row & 7)) * 16);
-        if (chunk * 8 < D) {
-          const T* src = cache + at;
-          const bool v = ok >> row & 1;
-          cp_async16(dst, v ? src : a.kv.base, v);
-          cp_async16(dst + kTile * DP * 2, v ? src + a.kv.lane_stride : a.kv.base, v);
-        }
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-      if (lo + i < hi) copy(i, lo + i);
-      cp_commit();
-    }
+    Window next = look_up(lo, b), now = next;
+    now.end = lo;
 
-    // ---- the products ----------------------------------------------------------------
-    const float to_base2 = a.scale * kLog2e;
-    int stage = 0;
-    for (uint32_t tile = lo; tile < hi; ++tile) {
-      if (tile >= end) {
-        do ++b;
-        while (first[b + 1] <= tile);
-        begin_request();
+    // The copies run kStages - 1 tiles ahead of the products.  One loop does both, so
+    // that no code stands twice: at the start of a kernel instructions come from
+    // memory too, and wait in line with the first tiles.
+    int stage = 0, into = 0;
+    for (uint32_t ahead = lo; ahead < hi + (S::kStages - 1); ++ahead) {
+      const uint32_t tile = ahead - (S::kStages - 1);  // whose products are taken, if ahead >= lo + kStages - 1
+      const bool takes = ahead >= lo + (S::kStages - 1);
+      if (ahead == lo || (takes && tile >= end)) {  // a request's first: its heads' rows
+        while (first[b + 1] <= (takes ? tile : lo)) ++b;
+        end = first[b + 1];
+        const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+            q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
+                          ? 0u
+                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
+          }
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
       }
-      cp_wait<S::kStages - 2>();
-      __syncwarp();
-      {  // the stage that the last step emptied
-        const int into = stage == 0 ? S::kStages - 1 : stage - 1;
-        if (tile + S::kStages - 1 < hi) copy(into, tile + S::kStages - 1);
-        cp_commit();
+      if (takes) {
+        cp_wait<S::kStages - 2>();
+        __syncwarp();
       }
+      if (ahead < hi) {  // into the stage that the last step emptied
+        if (ahead >= now.end) {
+          now = next;
+          next = look_up(now.end, now.b);
+        }
+        constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
+        const uint32_t t = (ahead - first[now.b]) * kTile + (lane & 15);
+        const int slot = static_cast<int>(t / static_cast<uint32_t>(bs)), off = static_cast<int>(t - slot * static_cast<uint32_t>(bs));
+        const int page = __shfl_sync(0xffffffffu, now.page, slot - now.slot);
+        const bool row_ok = off < __shfl_sync(0xffffffffu, now.tokens, slot - now.slot) && page >= 0 && page < a.kv.pages;
+        const long long row_at = row_ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
+        const uint32_t ok = __ballot_sync(0xffffffffu, row_ok) & 0xffffu;
+        if (lane == 0) valid_of[warp][into] = ok;
+        const uint32_t to = ring + into * S::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < kTile * kChunks / 32; ++i) {
+          const int row = (i * 32 + lane) / kChunks, chunk = (i * 32 + lane) % kChunks;
+          const long long at = __shfl_sync(0xffffffffu, row_at, row) + chunk * 8;
+          const uint32_t dst = to + row * DP * 2 + ((chunk ^ (row & 7)) * 16);
+          if (chunk * 8 < D) {
+            const T* src = cache + at;
+            const bool v = ok >> row & 1;
+            cp_async16(dst, v ? src : a.kv.base, v);
+            cp_async16(dst + kTile * DP * 2, v ? src + a.kv.lane_stride : a.kv.base, v);
+          }
+        }
+        into = into + 1 == S::kStages ? 0 : into + 1;
+      }
+      cp_commit();
+      if (!takes) continue;
       const uint32_t ok = valid_of[warp][stage];
       const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + kTile * DP * 2;
       float s[2][4] = {};
@@ -471,53 +466,63 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 
 // Adds up what the ranges left of a request that was cut.  There are no more cuts
 // than ranges: with few requests a CTA goes by a request, with many by a range's
-// begin, and is the one to work if that is the first cut of its request.  Its eight
-// warps share `heads_each` query heads; a warp takes eight parts at a time, whose
-// loads are in flight together.
-constexpr int kJoinWarps = 8, kJoinParts = 8;
+// begin, and is the one to work if that is the first cut of its request.  Its warps
+// share `units_each` units, 4 * LANES columns of a query head; LANES lanes take a part
+// and a warp 32 / LANES * kJoinParts parts at a time.  With LANES = 8 that is 160 for a
+// CTA: all parts of a request that lies over all SMs are in flight at once.
+constexpr int kJoinWarps = 8, kJoinParts = 5;
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kJoinWarps * 32)
-    attention_join_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w, int heads_each, bool by_cut) {
-  constexpr int kVecs = DP / 64;  // pairs of a lane
-  __shared__ __align__(16) float sum_o[kJoinWarps][DP];
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kJoinWarps * 32, 4)
+    attention_join_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w, int units_each, bool by_cut) {
+  constexpr int kColumns = 4 * LANES, kAtOnce = 32 / LANES;
+  __shared__ __align__(16) float sum_o[kJoinWarps][kColumns];
   __shared__ float sum_m[kJoinWarps], sum_l[kJoinWarps];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps_each = kJoinWarps / heads_each;
-  const int h = blockIdx.x * heads_each + warp / warps_each, mine = warp % warps_each;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps_each = kJoinWarps / units_each, mine = warp % warps_each;
   const int D = a.kv.dim, G = a.q.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
-  wait_for_parent();
-  const uint32_t tiles = w.first[a.req.requests];
-  if (tiles == 0) return;
-  const KvPlan plan = KvPlan::make(tiles, w.most_ranges, kLeastTiles);
-  int b = blockIdx.y;
-  if (by_cut) {
-    if (b + 1 >= plan.ranges) return;
-    b = w.begins[b + 1];
-  }
-  const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
-  if (f0 == f1) return;
-  const int r0 = plan.of(f0), r1 = plan.of(f1 - 1);
-  if (r0 == r1 || (by_cut && r0 != static_cast<int>(blockIdx.y))) return;  // finished where it was computed
-  float m = -INFINITY, l = 0.f;
-  float2 o[kVecs];
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) o[i] = make_float2(0.f, 0.f);
-  if (h < a.q.heads) {
-    // the first part may lie in its range's second place, the others lie in the first
-    const long long base = static_cast<long long>(h / G * per_head + h % G / kRowGroup) * w.rows + h % G % kRowGroup;
-    const long long step = static_cast<long long>(w.groups) * w.rows;
-    const int slot0 = plan.slot(r0, f0);
-    for (int r = r0 + mine * kJoinParts; r <= r1; r += warps_each * kJoinParts) {
-      float2 ml[kJoinParts], v[kJoinParts][kVecs];
+  const int chunks = (D + kColumns - 1) / kColumns, unit = blockIdx.x * units_each + warp / warps_each;
+  const int h = unit / chunks, d = unit % chunks * kColumns + lane % LANES * 4;
+  const bool on = h < a.q.heads && d < D;
+  // the place of head h's row in a part, and the parts' distance
+  const long long base = static_cast<long long>(h / G * per_head + h % G / kRowGroup) * w.rows + h % G % kRowGroup;
+  const long long step = static_cast<long long>(w.groups) * w.rows;
+  // The first pass has nothing to add: it brings the code in while the parts are
+  // still being computed.
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    int b = blockIdx.y, r0 = 0, r1 = -1, slot0 = 0;
+    if (pass == 1) {
+      wait_for_parent();
+      const uint32_t tiles = w.first[a.req.requests];
+      if (tiles == 0) return;
+      const KvPlan plan = KvPlan::make(tiles, w.most_ranges, kLeastTiles);
+      if (by_cut) {
+        if (b + 1 >= plan.ranges) return;
+        b = w.begins[b + 1];
+      }
+      const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
+      if (f0 == f1) return;
+      r0 = plan.of(f0);
+      r1 = plan.of(f1 - 1);
+      if (r0 == r1 || (by_cut && r0 != static_cast<int>(blockIdx.y))) return;  // finished where it was computed
+      // the first part may lie in its range's second place, the others lie in the first
+      slot0 = plan.slot(r0, f0);
+    }
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    int r = r0 + mine * kAtOnce * kJoinParts + lane / LANES;
+    do {
+      float2 ml[kJoinParts];
+      float4 v[kJoinParts];
 #pragma unroll
       for (int k = 0; k < kJoinParts; ++k) {
-        const long long at = base + step * (r + k == r0 ? slot0 : 2 * (r + k));
+        const int x = r + kAtOnce * k;
+        const long long at = base + step * (x == r0 ? slot0 : 2 * x);
         ml[k] = make_float2(-INFINITY, 0.f);
-        if (r + k <= r1) ml[k] = w.part_ml[at];
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-          v[k][i] = make_float2(0.f, 0.f);
-          if (r + k <= r1 && i * 64 + lane * 2 < D) v[k][i] = *reinterpret_cast<const float2*>(w.part_o + at * D + i * 64 + lane * 2);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (x <= r1 && on) {
+          ml[k] = w.part_ml[at];
+          v[k] = *reinterpret_cast<const float4*>(w.part_o + at * D + d);
         }
       }
       float now = m;
@@ -526,50 +531,54 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
       const float ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref);
       m = now;
       l *= c;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) o[i].x *= c, o[i].y *= c;
+      o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
 #pragma unroll
       for (int k = 0; k < kJoinParts; ++k) {
         const float p = ex2(ml[k].x - ref);
         l += ml[k].y * p;
+        o = make_float4(o.x + v[k].x * p, o.y + v[k].y * p, o.z + v[k].z * p, o.w + v[k].w * p);
+      }
+      r += warps_each * kAtOnce * kJoinParts;
+    } while (r - lane / LANES <= r1);
+    // the groups of lanes, then the warps
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) o[i].x += v[k][i].x * p, o[i].y += v[k][i].y * p;
+    for (int x = LANES; x < 32; x *= 2) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, x), now = fmaxf(m, m2), ref = now == -INFINITY ? 0.f : now;
+      const float p = ex2(m - ref), p2 = ex2(m2 - ref);
+      m = now;
+      l = l * p + __shfl_xor_sync(0xffffffffu, l, x) * p2;
+      o.x = o.x * p + __shfl_xor_sync(0xffffffffu, o.x, x) * p2;
+      o.y = o.y * p + __shfl_xor_sync(0xffffffffu, o.y, x) * p2;
+      o.z = o.z * p + __shfl_xor_sync(0xffffffffu, o.z, x) * p2;
+      o.w = o.w * p + __shfl_xor_sync(0xffffffffu, o.w, x) * p2;
+    }
+    if (warps_each > 1) {
+      __syncthreads();  // the first pass' sums have been read
+      if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
+      if (lane < LANES) *reinterpret_cast<float4*>(&sum_o[warp][lane * 4]) = o;
+      __syncthreads();
+      const int w0 = warp - mine;
+      float top = -INFINITY;
+      for (int i = 0; i < warps_each; ++i) top = fmaxf(top, sum_m[w0 + i]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      m = top;
+      l = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < warps_each; ++i) {
+        const float p = ex2(sum_m[w0 + i] - ref);
+        const float4 v = *reinterpret_cast<const float4*>(&sum_o[w0 + i][lane % LANES * 4]);
+        l += p * sum_l[w0 + i];
+        o = make_float4(o.x + v.x * p, o.y + v.y * p, o.z + v.z * p, o.w + v.w * p);
       }
     }
+    if (pass == 0 || mine != 0 || lane >= LANES || !on) continue;
+    const long long row = static_cast<long long>(b) * a.q.heads + h;
+    const uint32_t lo = l == 0.f ? 0u : Type<T>::pack(o.x / l, o.y / l), hi = l == 0.f ? 0u : Type<T>::pack(o.z / l, o.w / l);
+    T* out = static_cast<T*>(a.out) + row * D + d;
+    *reinterpret_cast<uint32_t*>(out) = lo;
+    *reinterpret_cast<uint32_t*>(out + 2) = hi;
+    if (d == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + lg2(l)) * kLn2;
   }
-  if (warps_each > 1) {
-    if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) *reinterpret_cast<float2*>(&sum_o[warp][i * 64 + lane * 2]) = o[i];
-    __syncthreads();
-    if (mine != 0) return;
-    float top = -INFINITY;
-    for (int i = 0; i < warps_each; ++i) top = fmaxf(top, sum_m[warp + i]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    m = top;
-    l = 0.f;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) o[i] = make_float2(0.f, 0.f);
-    for (int k = 0; k < warps_each; ++k) {
-      const float p = ex2(sum_m[warp + k] - ref);
-      l += p * sum_l[warp + k];
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const float2 v = *reinterpret_cast<const float2*>(&sum_o[warp + k][i * 64 + lane * 2]);
-        o[i].x += v.x * p;
-        o[i].y += v.y * p;
-      }
-    }
-  }
-  if (h >= a.q.heads) return;
-  const long long row = static_cast<long long>(b) * a.q.heads + h;
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int d = i * 64 + lane * 2;
-    if (d < D)
-      *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + row * D + d) = l == 0.f ? 0u : Type<T>::pack(o[i].x / l, o[i].y / l);
-  }
-  if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
 // A warp for each block: the tiles' sums of every head, weighed by the head's total.
@@ -657,14 +666,22 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
   kernel<<<sms, threads, smem, stream>>>(a, w);
   rc = cudaGetLastError();
   if (rc != cudaSuccess) return rc;
-  // as many warps for a head as leave four CTAs to an SM
   const bool by_cut = a.req.requests >= w.most_ranges;
   const int items = by_cut ? w.most_ranges - 1 : a.req.requests;
   if (items == 0) return cudaSuccess;
-  int heads_each = 1;
-  while (heads_each < kJoinWarps && static_cast<int64_t>(items) * ((a.q.heads + heads_each - 1) / heads_each) > 4 * sms) heads_each *= 2;
-  return launch_after(attention_join_kernel<T, DP>, dim3((a.q.heads + heads_each - 1) / heads_each, items), kJoinWarps * 32,
-                      stream, a, w, heads_each, by_cut);
+  // narrow units while the CTAs fit beside the attention's, else whole rows, and
+  // as many warps for a unit as leave two CTAs to an SM
+  auto join = attention_join_kernel<T, 8>;
+  int units = a.q.heads * ((a.kv.dim + 31) / 32), each = 1;
+  auto ctas = [&] { return static_cast<int64_t>(items) * ((units + each - 1) / each); };
+  while (each < kJoinWarps && ctas() > sms) each *= 2;
+  if (ctas() > sms) {
+    join = attention_join_kernel<T, 32>;
+    units = a.q.heads * ((a.kv.dim + 127) / 128);
+    each = 1;
+    while (each < kJoinWarps && ctas() > 2 * sms) each *= 2;
+  }
+  return launch_after(join, dim3((units + each - 1) / each, items), kJoinWarps * 32, stream, a, w, each, by_cut);
 }
 
 template <typename T>
