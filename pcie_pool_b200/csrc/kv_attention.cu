@@ -34,7 +34,7 @@ namespace ppb {
 namespace {
 
 constexpr int kTile = 16;      // tokens of a step; the mass is gathered by tiles
-constexpr int kLeastTiles = 2; // of a range: shorter ones cost more to join than they save
+constexpr int kLeastTiles = 1; // of a range: two cost a short request 1 us more, four 3 us
 constexpr int kMostRequests = 4096;
 constexpr int kRowGroup = 16;  // query heads of one warp at most
 constexpr float kLog2e = 1.4426950408889634f;
@@ -59,6 +59,7 @@ struct Work {
   int* begins;          // [ranges]: the request of a range's first tile
   float* z;             // [requests, max_tiles, heads]: log2 of a tile's sum, or null
   int max_tiles;        // of a request
+  int mass_ctas;        // of a request
   int most_ranges;
   int groups;           // kv_heads * row groups
   int rows;             // of a group's partial result: 8 or 16
@@ -209,7 +210,8 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
   __shared__ uint32_t valid_of[S::kWarps][S::kStages];
   uint32_t* first = reinterpret_cast<uint32_t*>(smem + S::kRingBytes);
   int* lens = reinterpret_cast<int*>(first + a.req.requests + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
   const int D = a.kv.dim, bs = a.kv.block, G = a.q.heads / a.kv.kv_heads, n = a.req.requests;
   launch_dependents();
   if (D < DP)  // what the copies leave of a row stays zero
@@ -226,18 +228,17 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
     }
   const KvPlan plan = KvPlan::make(first[n], w.most_ranges, kLeastTiles);
   if (plan.tiles == 0) return;
-  const long long units = static_cast<long long>(plan.ranges) * w.groups;
+  const uint32_t units = static_cast<uint32_t>(plan.ranges) * w.groups;
   // few units: one to a CTA before two
-  const int per_cta = static_cast<int>(min(static_cast<long long>(S::kWarps), (units + gridDim.x - 1) / gridDim.x));
+  const uint32_t per_cta = min(static_cast<uint32_t>(S::kWarps), (units + gridDim.x - 1) / gridDim.x);
   if (warp >= per_cta) return;
   const uint32_t ring = dev::smem_u32(smem) + warp * S::kStages * S::kStageBytes;
 
-  for (long long unit = static_cast<long long>(blockIdx.x) * per_cta + warp; unit < units;
-       unit += static_cast<long long>(gridDim.x) * per_cta) {
-    const int r = static_cast<int>(unit / w.groups), group = static_cast<int>(unit % w.groups);
+  for (uint32_t unit = blockIdx.x * per_cta + warp; unit < units; unit += gridDim.x * per_cta) {
+    const int r = static_cast<int>(unit / w.groups), group = static_cast<int>(unit - r * w.groups);
     const int per_head = (G + kRowGroup - 1) / kRowGroup, g = group / per_head, row0 = group % per_head * kRowGroup;
     const int rows = min(kRowGroup, G - row0);
-    const uint32_t lo = static_cast<uint32_t>(plan.begin(r)), hi = static_cast<uint32_t>(plan.begin(r + 1));
+    const uint32_t lo = plan.begin(r), hi = plan.begin(r + 1);
     const T* cache = static_cast<const T*>(a.kv.base) + g * a.kv.head_stride;
 
     float o[DP / 8][4], m[2], l[2];
@@ -464,140 +465,185 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
   }
 }
 
+constexpr int kJoinWarps = 8, kJoinParts = 5;
+
+struct Join {
+  uint32_t ctas;       // that join; the others add the mass
+  uint32_t ctas_each;  // of a request, or of a cut
+  int units_each;
+  bool by_cut;
+};
+
+// The mass of kMassBlocks blocks of a request, a warp for each: the sums of its
+// tiles for every head (they lie together) over the heads' totals.  The totals of
+// a request that was cut are taken from its parts, eight lanes for a head, since
+// the join beside it only writes them now; the tiles' sums and the old mass are on
+// their way meanwhile.
+constexpr int kMassBlocks = kJoinWarps, kMassHeads = 1024, kMassAhead = 8;
+
+__device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, uint32_t cta) {
+  __shared__ float total[kMassHeads];
+  const int b = cta / w.mass_ctas, j = (cta - b * w.mass_ctas) * kMassBlocks + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32, H = a.q.heads, per = a.kv.block / kTile;
+  const int G = H / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
+  wait_for_parent();
+  const uint32_t f0 = w.first[b], f1 = w.first[b + 1];  // a request's tiles are all its blocks'
+  const int t0 = j * per, blocks = (f1 - f0 + per - 1) / per;
+  if (j - static_cast<int>(threadIdx.x / 32) >= blocks) return;
+  const int count = j < blocks ? min(per, static_cast<int>(f1 - f0) - t0) * H : 0;
+  const float* z = w.z + (static_cast<long long>(b) * w.max_tiles + t0) * H;
+  float* mass = a.mass + b * a.mass_stride + j;
+  float ahead[kMassAhead], old = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMassAhead; ++i) ahead[i] = i * 32 + lane < count ? z[i * 32 + lane] : -INFINITY;
+  if (j < blocks) old = *mass;
+  const KvPlan plan = KvPlan::make(w.first[a.req.requests], w.most_ranges, kLeastTiles);
+  const int r0 = plan.of(f0), r1 = plan.of(f1 - 1), slot0 = plan.slot(r0, f0);
+  for (int h = threadIdx.x / 8; h < (H + 3) / 4 * 4; h += kJoinWarps * 4) {  // whole warps: they shuffle
+    float m = -INFINITY, l = 0.f;
+    if (r0 == r1) {
+      if (h < H) m = a.lse[static_cast<long long>(b) * H + h] * kLog2e, l = 1.f;
+    } else {
+      const long long base = static_cast<long long>(h / G * per_head + h % G / kRowGroup) * w.rows + h % G % kRowGroup;
+      const long long step = static_cast<long long>(w.groups) * w.rows;
+#pragma unroll 4
+      for (int r = r0 + (lane & 7); r <= r1; r += 8) {
+        const float2 ml = h < H ? w.part_ml[base + step * (r == r0 ? slot0 : 2 * r)] : make_float2(-INFINITY, 0.f);
+        const float now = fmaxf(m, ml.x), ref = now == -INFINITY ? 0.f : now;
+        l = l * ex2(m - ref) + ml.y * ex2(ml.x - ref);
+        m = now;
+      }
+#pragma unroll
+      for (int x = 4; x > 0; x /= 2) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, x), now = fmaxf(m, m2), ref = now == -INFINITY ? 0.f : now;
+        l = l * ex2(m - ref) + __shfl_xor_sync(0xffffffffu, l, x) * ex2(m2 - ref);
+        m = now;
+      }
+    }
+    if ((lane & 7) == 0 && h < H) total[h] = l == 0.f ? -INFINITY : m + lg2(l);
+  }
+  __syncthreads();
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMassAhead; ++i)
+    if (ahead[i] != -INFINITY) sum += ex2(ahead[i] - total[(i * 32 + lane) % H]);
+  for (int i = kMassAhead * 32 + lane; i < count; i += 32) {
+    const float v = z[i];
+    if (v != -INFINITY) sum += ex2(v - total[i % H]);
+  }
+  sum = dev::warp_sum(sum);
+  if (j < blocks && lane == 0) *mass = old + sum;
+}
+
 // Adds up what the ranges left of a request that was cut.  There are no more cuts
 // than ranges: with few requests a CTA goes by a request, with many by a range's
 // begin, and is the one to work if that is the first cut of its request.  Its warps
 // share `units_each` units, 4 * LANES columns of a query head; LANES lanes take a part
 // and a warp 32 / LANES * kJoinParts parts at a time.  With LANES = 8 that is 160 for a
 // CTA: all parts of a request that lies over all SMs are in flight at once.
-constexpr int kJoinWarps = 8, kJoinParts = 5;
-
-template <typename T, int LANES>
+template <typename T, int LANES, bool MASS>
 __global__ void __launch_bounds__(kJoinWarps * 32, 4)
-    attention_join_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w, int units_each, bool by_cut) {
+    attention_join_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w, const __grid_constant__ Join j) {
+  if (MASS && blockIdx.x >= j.ctas) {
+    add_mass(a, w, blockIdx.x - j.ctas);
+    return;
+  }
+  const int units_each = j.units_each, item = blockIdx.x / j.ctas_each;
+  const bool by_cut = j.by_cut;
   constexpr int kColumns = 4 * LANES, kAtOnce = 32 / LANES;
   __shared__ __align__(16) float sum_o[kJoinWarps][kColumns];
   __shared__ float sum_m[kJoinWarps], sum_l[kJoinWarps];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps_each = kJoinWarps / units_each, mine = warp % warps_each;
   const int D = a.kv.dim, G = a.q.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
-  const int chunks = (D + kColumns - 1) / kColumns, unit = blockIdx.x * units_each + warp / warps_each;
+  const int chunks = (D + kColumns - 1) / kColumns, unit = (blockIdx.x - item * j.ctas_each) * units_each + warp / warps_each;
   const int h = unit / chunks, d = unit % chunks * kColumns + lane % LANES * 4;
   const bool on = h < a.q.heads && d < D;
   // the place of head h's row in a part, and the parts' distance
   const long long base = static_cast<long long>(h / G * per_head + h % G / kRowGroup) * w.rows + h % G % kRowGroup;
   const long long step = static_cast<long long>(w.groups) * w.rows;
-  // The first pass has nothing to add: it brings the code in while the parts are
-  // still being computed.
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    int b = blockIdx.y, r0 = 0, r1 = -1, slot0 = 0;
-    if (pass == 1) {
-      wait_for_parent();
-      const uint32_t tiles = w.first[a.req.requests];
-      if (tiles == 0) return;
-      const KvPlan plan = KvPlan::make(tiles, w.most_ranges, kLeastTiles);
-      if (by_cut) {
-        if (b + 1 >= plan.ranges) return;
-        b = w.begins[b + 1];
-      }
-      const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
-      if (f0 == f1) return;
-      r0 = plan.of(f0);
-      r1 = plan.of(f1 - 1);
-      if (r0 == r1 || (by_cut && r0 != static_cast<int>(blockIdx.y))) return;  // finished where it was computed
-      // the first part may lie in its range's second place, the others lie in the first
-      slot0 = plan.slot(r0, f0);
-    }
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    int r = r0 + mine * kAtOnce * kJoinParts + lane / LANES;
-    do {
-      float2 ml[kJoinParts];
-      float4 v[kJoinParts];
-#pragma unroll
-      for (int k = 0; k < kJoinParts; ++k) {
-        const int x = r + kAtOnce * k;
-        const long long at = base + step * (x == r0 ? slot0 : 2 * x);
-        ml[k] = make_float2(-INFINITY, 0.f);
-        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (x <= r1 && on) {
-          ml[k] = w.part_ml[at];
-          v[k] = *reinterpret_cast<const float4*>(w.part_o + at * D + d);
-        }
-      }
-      float now = m;
-#pragma unroll
-      for (int k = 0; k < kJoinParts; ++k) now = fmaxf(now, ml[k].x);
-      const float ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref);
-      m = now;
-      l *= c;
-      o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
-#pragma unroll
-      for (int k = 0; k < kJoinParts; ++k) {
-        const float p = ex2(ml[k].x - ref);
-        l += ml[k].y * p;
-        o = make_float4(o.x + v[k].x * p, o.y + v[k].y * p, o.z + v[k].z * p, o.w + v[k].w * p);
-      }
-      r += warps_each * kAtOnce * kJoinParts;
-    } while (r - lane / LANES <= r1);
-    // the groups of lanes, then the warps
-#pragma unroll
-    for (int x = LANES; x < 32; x *= 2) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, x), now = fmaxf(m, m2), ref = now == -INFINITY ? 0.f : now;
-      const float p = ex2(m - ref), p2 = ex2(m2 - ref);
-      m = now;
-      l = l * p + __shfl_xor_sync(0xffffffffu, l, x) * p2;
-      o.x = o.x * p + __shfl_xor_sync(0xffffffffu, o.x, x) * p2;
-      o.y = o.y * p + __shfl_xor_sync(0xffffffffu, o.y, x) * p2;
-      o.z = o.z * p + __shfl_xor_sync(0xffffffffu, o.z, x) * p2;
-      o.w = o.w * p + __shfl_xor_sync(0xffffffffu, o.w, x) * p2;
-    }
-    if (warps_each > 1) {
-      __syncthreads();  // the first pass' sums have been read
-      if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
-      if (lane < LANES) *reinterpret_cast<float4*>(&sum_o[warp][lane * 4]) = o;
-      __syncthreads();
-      const int w0 = warp - mine;
-      float top = -INFINITY;
-      for (int i = 0; i < warps_each; ++i) top = fmaxf(top, sum_m[w0 + i]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      m = top;
-      l = 0.f;
-      o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = 0; i < warps_each; ++i) {
-        const float p = ex2(sum_m[w0 + i] - ref);
-        const float4 v = *reinterpret_cast<const float4*>(&sum_o[w0 + i][lane % LANES * 4]);
-        l += p * sum_l[w0 + i];
-        o = make_float4(o.x + v.x * p, o.y + v.y * p, o.z + v.z * p, o.w + v.w * p);
-      }
-    }
-    if (pass == 0 || mine != 0 || lane >= LANES || !on) continue;
-    const long long row = static_cast<long long>(b) * a.q.heads + h;
-    const uint32_t lo = l == 0.f ? 0u : Type<T>::pack(o.x / l, o.y / l), hi = l == 0.f ? 0u : Type<T>::pack(o.z / l, o.w / l);
-    T* out = static_cast<T*>(a.out) + row * D + d;
-    *reinterpret_cast<uint32_t*>(out) = lo;
-    *reinterpret_cast<uint32_t*>(out + 2) = hi;
-    if (d == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + lg2(l)) * kLn2;
-  }
-}
-
-// A warp for each block: the tiles' sums of every head, weighed by the head's total.
-__global__ void __launch_bounds__(128) mass_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w) {
-  const int b = blockIdx.y, j = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
   wait_for_parent();
-  const int len = length_of(a, b);
-  if (j >= (len + a.kv.block - 1) / a.kv.block) return;
-  const int per = a.kv.block / kTile, t0 = j * per, t1 = min(t0 + per, (len + kTile - 1) / kTile);
-  float sum = 0.f;
-  for (int h = lane; h < a.q.heads; h += 32) {
-    const float total = a.lse[static_cast<long long>(b) * a.q.heads + h] * kLog2e;
-    for (int t = t0; t < t1; ++t) {
-      const float v = w.z[(static_cast<long long>(b) * w.max_tiles + t) * a.q.heads + h];
-      sum += v == -INFINITY ? 0.f : ex2(v - total);
+  const uint32_t tiles = w.first[a.req.requests];
+  if (tiles == 0) return;
+  const KvPlan plan = KvPlan::make(tiles, w.most_ranges, kLeastTiles);
+  int b = item;
+  if (by_cut) {
+    if (b + 1 >= plan.ranges) return;
+    b = w.begins[b + 1];
+  }
+  const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
+  if (f0 == f1) return;
+  const int r0 = plan.of(f0), r1 = plan.of(f1 - 1);
+  if (r0 == r1 || (by_cut && r0 != item)) return;  // finished where it was computed
+  const int slot0 = plan.slot(r0, f0);  // the first part may lie in its range's second place, the others lie in the first
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  int r = r0 + mine * kAtOnce * kJoinParts + lane / LANES;
+  do {
+    float2 ml[kJoinParts];
+    float4 v[kJoinParts];
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) {
+      const int x = r + kAtOnce * k;
+      const long long at = base + step * (x == r0 ? slot0 : 2 * x);
+      ml[k] = make_float2(-INFINITY, 0.f);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (x <= r1 && on) {
+        ml[k] = w.part_ml[at];
+        v[k] = *reinterpret_cast<const float4*>(w.part_o + at * D + d);
+      }
+    }
+    float now = m;
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) now = fmaxf(now, ml[k].x);
+    const float ref = now == -INFINITY ? 0.f : now, c = ex2(m - ref);
+    m = now;
+    l *= c;
+    o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) {
+      const float p = ex2(ml[k].x - ref);
+      l += ml[k].y * p;
+      o = make_float4(o.x + v[k].x * p, o.y + v[k].y * p, o.z + v[k].z * p, o.w + v[k].w * p);
+    }
+    r += warps_each * kAtOnce * kJoinParts;
+  } while (r - lane / LANES <= r1);
+  // the groups of lanes, then the warps
+#pragma unroll
+  for (int x = LANES; x < 32; x *= 2) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, x), now = fmaxf(m, m2), ref = now == -INFINITY ? 0.f : now;
+    const float p = ex2(m - ref), p2 = ex2(m2 - ref);
+    m = now;
+    l = l * p + __shfl_xor_sync(0xffffffffu, l, x) * p2;
+    o.x = o.x * p + __shfl_xor_sync(0xffffffffu, o.x, x) * p2;
+    o.y = o.y * p + __shfl_xor_sync(0xffffffffu, o.y, x) * p2;
+    o.z = o.z * p + __shfl_xor_sync(0xffffffffu, o.z, x) * p2;
+    o.w = o.w * p + __shfl_xor_sync(0xffffffffu, o.w, x) * p2;
+  }
+  if (warps_each > 1) {
+    if (lane == 0) sum_m[warp] = m, sum_l[warp] = l;
+    if (lane < LANES) *reinterpret_cast<float4*>(&sum_o[warp][lane * 4]) = o;
+    __syncthreads();
+    const int w0 = warp - mine;
+    float top = -INFINITY;
+    for (int i = 0; i < warps_each; ++i) top = fmaxf(top, sum_m[w0 + i]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    m = top;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < warps_each; ++i) {
+      const float p = ex2(sum_m[w0 + i] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(&sum_o[w0 + i][lane % LANES * 4]);
+      l += p * sum_l[w0 + i];
+      o = make_float4(o.x + v.x * p, o.y + v.y * p, o.z + v.z * p, o.w + v.w * p);
     }
   }
-  sum = dev::warp_sum(sum);
-  if (lane == 0) a.mass[b * a.mass_stride + j] += sum;
+  if (mine != 0 || lane >= LANES || !on) return;
+  const long long row = static_cast<long long>(b) * a.q.heads + h;
+  const uint32_t lo = l == 0.f ? 0u : Type<T>::pack(o.x / l, o.y / l), hi = l == 0.f ? 0u : Type<T>::pack(o.z / l, o.w / l);
+  T* out = static_cast<T*>(a.out) + row * D + d;
+  *reinterpret_cast<uint32_t*>(out) = lo;
+  *reinterpret_cast<uint32_t*>(out + 2) = hi;
+  if (d == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
 int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -612,6 +658,7 @@ uint64_t lay_out(int requests, int width, int block, int heads, int kv_heads, in
   w.rows = G <= 8 ? 8 : 16;
   w.most_ranges = warps / w.groups > 0 ? warps / w.groups : 1;
   w.max_tiles = static_cast<int>((static_cast<int64_t>(width) * block + kTile - 1) / kTile);
+  w.mass_ctas = mass ? (width + kMassBlocks - 1) / kMassBlocks : 0;
   const uint64_t parts = 2ull * w.most_ranges * w.groups * w.rows;
   uint8_t* p = static_cast<uint8_t*>(base);
   uint64_t at = 0;
@@ -666,22 +713,28 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
   kernel<<<sms, threads, smem, stream>>>(a, w);
   rc = cudaGetLastError();
   if (rc != cudaSuccess) return rc;
-  const bool by_cut = a.req.requests >= w.most_ranges;
-  const int items = by_cut ? w.most_ranges - 1 : a.req.requests;
-  if (items == 0) return cudaSuccess;
+  Join j;
+  j.by_cut = a.req.requests >= w.most_ranges;
+  const uint32_t items = j.by_cut ? w.most_ranges - 1 : a.req.requests;
   // narrow units while the CTAs fit beside the attention's, else whole rows, and
   // as many warps for a unit as leave two CTAs to an SM
-  auto join = attention_join_kernel<T, 8>;
-  int units = a.q.heads * ((a.kv.dim + 31) / 32), each = 1;
-  auto ctas = [&] { return static_cast<int64_t>(items) * ((units + each - 1) / each); };
-  while (each < kJoinWarps && ctas() > sms) each *= 2;
-  if (ctas() > sms) {
-    join = attention_join_kernel<T, 32>;
-    units = a.q.heads * ((a.kv.dim + 127) / 128);
-    each = 1;
-    while (each < kJoinWarps && ctas() > 2 * sms) each *= 2;
+  auto join = w.z ? attention_join_kernel<T, 8, true> : attention_join_kernel<T, 8, false>;
+  auto share_out = [&](int columns, int64_t most) {
+    const int units = a.q.heads * ((a.kv.dim + columns - 1) / columns);
+    for (j.units_each = 1;; j.units_each *= 2) {
+      j.ctas_each = (units + j.units_each - 1) / j.units_each;
+      if (j.units_each == kJoinWarps || static_cast<int64_t>(items) * j.ctas_each <= most) break;
+    }
+    j.ctas = items * j.ctas_each;
+    return static_cast<int64_t>(items) * j.ctas_each <= most;
+  };
+  if (!share_out(32, sms)) {
+    join = w.z ? attention_join_kernel<T, 32, true> : attention_join_kernel<T, 32, false>;
+    share_out(128, 2 * sms);
   }
-  return launch_after(join, dim3((units + each - 1) / each, items), kJoinWarps * 32, stream, a, w, each, by_cut);
+  const uint32_t ctas = j.ctas + static_cast<uint32_t>(a.req.requests) * w.mass_ctas;
+  if (ctas == 0) return cudaSuccess;
+  return launch_after(join, dim3(ctas), kJoinWarps * 32, stream, a, w, j);
 }
 
 template <typename T>
@@ -712,8 +765,6 @@ cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream) {
   lay_out(a.req.requests, a.req.width, a.kv.block, a.q.heads, a.kv.kv_heads, a.kv.dim, a.mass != nullptr, sms, a.work, w);
   rc = a.kv.type == kKvBf16 ? launch<__nv_bfloat16>(a, w, sms, device, stream)
                              : launch<__half>(a, w, sms, device, stream);
-  if (rc == cudaSuccess && a.mass && a.req.width)
-    rc = launch_after(mass_kernel, dim3((a.req.width + 3) / 4, a.req.requests), 128, stream, a, w);
   return rc;
 }
 

@@ -37,6 +37,7 @@ from .._native import native
 MAX_REQUESTS = 4096
 MAX_DIM = 256
 MAX_BLOCK = 65536
+MAX_MASS_HEADS = 1024
 
 
 def _torch():
@@ -132,15 +133,12 @@ def _query(torch, q, device: int, dtype, dim: int, kv_heads: int, requests: int)
     return q, (at, row, head, heads)
 
 
-def _overlap(a, b) -> bool:
-    def span(t):
-        lo = t.data_ptr()
-        return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-    if not a.numel() or not b.numel():
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+def _overlap(t, cache) -> bool:
+    """Whether a contiguous 16-bit tensor shares memory with the span of a cache (its arguments)."""
+    at, lane, page, token, head, pages, block, heads, dim, _ = cache
+    end = at + 2 * (lane + max(pages - 1, 0) * page + (block - 1) * token + (heads - 1) * head + dim)
+    low = t.data_ptr()
+    return low < end and at < low + 2 * t.numel()
 
 
 def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=None, mass=None, out=None,
@@ -163,7 +161,7 @@ def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=N
     ``mass`` fp32 [requests, blocks of the table] is added to in place: the
     attention weight that the heads gave to each block, summed over heads and
     tokens, so a request's row grows by ``heads`` in all.  It needs a block size
-    that is a multiple of 16 and takes no ``blocks``.
+    that is a multiple of 16 and at most 1024 heads, and takes no ``blocks``.
     """
     torch = _torch()
     cache = _cache(torch, kv)
@@ -182,6 +180,8 @@ def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=N
     if mass is not None:
         if blocks is not None:
             raise ValueError("mass is gathered over all blocks: it takes no blocks=")
+        if heads > MAX_MASS_HEADS:
+            raise ValueError(f"mass takes at most {MAX_MASS_HEADS} heads")
         if block % 16:
             raise ValueError("mass needs a block size that is a multiple of 16")
         if mass.dtype != torch.float32 or mass.get_device() != index or mass.shape != block_table.shape:
@@ -194,7 +194,9 @@ def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=N
         if (out.dtype != q.dtype or out.get_device() != index or out.shape != q.shape or not out.is_contiguous()
                 or out.data_ptr() % 4):
             raise ValueError("out must be contiguous, like q, on a 4-byte boundary")
-        if _overlap(out, q) or _overlap(out, kv):
+        at, row, head, _ = query
+        size = 2 * (max(n - 1, 0) * row + (heads - 1) * head + dim)
+        if _overlap(out, cache) or (out.data_ptr() < at + size and at < out.data_ptr() + out.numel() * 2):
             raise ValueError("out must not overlap q or kv")
     stream = _runs(torch, kv, q)
     if out is None:
@@ -228,7 +230,7 @@ def paged_kv_bounds(kv, block_table, context_lens, bounds, *, new_tokens=None):
     if (bounds.dtype != kv.dtype or bounds.get_device() != index or bounds.shape != (pages, heads, 2, dim)
             or not bounds.is_contiguous() or bounds.data_ptr() % 16):
         raise ValueError("bounds must be contiguous [pages, kv_heads, 2, dim] in the cache's type, on a 16-byte boundary")
-    if _overlap(bounds, kv):
+    if _overlap(bounds, cache):
         raise ValueError("bounds must not overlap kv")
     since = -1 if new_tokens is None else _int(new_tokens, "new_tokens", 0)
     stream = _runs(torch, kv, bounds)

@@ -19,9 +19,9 @@ using ppb::KvPlan;
     }                                                                \
   } while (0)
 
-static void check(const std::vector<int64_t>& tiles, int most, int least) {
-  std::vector<int64_t> first{0};
-  for (int64_t t : tiles) first.push_back(first.back() + t);
+static void check(const std::vector<uint32_t>& tiles, int most, int least) {
+  std::vector<uint32_t> first{0};
+  for (uint32_t t : tiles) first.push_back(first.back() + t);
   const KvPlan p = KvPlan::make(first.back(), most, least);
   CHECK(p.ranges >= 1 && p.ranges <= most);
   if (p.tiles == 0) return;
@@ -30,7 +30,7 @@ static void check(const std::vector<int64_t>& tiles, int most, int least) {
   std::set<int> slots;
   size_t b = 0;
   for (int r = 0; r < p.ranges; ++r) {
-    const int64_t lo = p.begin(r), hi = p.begin(r + 1);
+    const uint32_t lo = p.begin(r), hi = p.begin(r + 1);
     CHECK(lo < hi);  // ranges are never more than tiles
     CHECK(p.of(lo) == r && p.of(hi - 1) == r);
     while (first[b + 1] <= lo) ++b;
@@ -55,12 +55,13 @@ static void check(const std::vector<int64_t>& tiles, int most, int least) {
 int main() {
   std::mt19937 rng(1);
   for (int i = 0; i < 4000; ++i) {
-    std::vector<int64_t> t(1 + rng() % (i % 4 ? 20 : 900));
+    std::vector<uint32_t> t(1 + rng() % (i % 4 ? 20 : 900));
     for (auto& v : t) v = rng() % 3 == 0 ? 0 : 1 + rng() % (1 << rng() % 14);
     check(t, 1 + static_cast<int>(rng() % 1200), 1 + static_cast<int>(rng() % 4));
   }
-  check({(1ll << 32) - 1}, 1184, 2);
-  check({1, (1ll << 32) - 3, 1}, 1184, 2);
+  check({1u << 31}, 1184, 2);
+  check({1, (1u << 31) - 2, 1}, 1184, 2);
+  check({(1u << 31) - 1}, 32767, 1);
   check({0, 0, 1, 0}, 148, 2);
   check({0}, 148, 2);
   std::printf("kv_plan_test: ok\n");

@@ -47,6 +47,7 @@ BAD_ATTENTION = {
     "mass type": (lambda a: dict(mass=torch.zeros(a["block_table"].shape, dtype=torch.float64)), "mass must be"),
     "mass shape": (lambda a: dict(mass=torch.zeros(2, 1)), "mass must be"),
     "mass rows": (lambda a: dict(mass=torch.zeros(1, a["block_table"].shape[1]).expand(2, -1)), "rows of their own"),
+    "mass heads": (lambda a: dict(q=a["q"][:, :1].expand(-1, 1026, -1), mass=torch.zeros(a["block_table"].shape)), "at most 1024"),
     "mass and blocks": (lambda a: dict(mass=torch.zeros(a["block_table"].shape),
                                        blocks=torch.zeros(2, 2, 1, dtype=torch.int32)), "takes no blocks"),
     "blocks type": (lambda a: dict(blocks=torch.zeros(2, 2, 1, dtype=torch.int64)), "blocks must be"),
