@@ -34,7 +34,6 @@ namespace ppb {
 namespace {
 
 constexpr int kTile = 16;      // tokens of a step; the mass is gathered by tiles
-constexpr int kLeastTiles = 1; // of a range: two cost a short request 1 us more, four 3 us
 constexpr int kMostRequests = 4096;
 constexpr int kRowGroup = 16;  // query heads of one warp at most
 constexpr float kLog2e = 1.4426950408889634f;
@@ -61,7 +60,10 @@ struct Work {
   int max_tiles;        // of a request
   int mass_ctas;        // of a request
   int most_ranges;
-  int groups;           // kv_heads * row groups
+  int shared;           // query heads of a key head
+  int groups_each;      // row groups of a key head
+  int groups;           // of all key heads
+  FastDiv by_ranges, by_block, by_groups, by_groups_each;
   int rows;             // of a group's partial result: 8 or 16
 };
 
@@ -149,19 +151,17 @@ __device__ __forceinline__ int length_of(const KvAttention& a, int b) {
   return max(0, static_cast<int>(min(static_cast<long long>(a.req.lens[b]), most)));
 }
 
-// Blocks of a request that are read: all that hold tokens, or the listed ones.
-__device__ __forceinline__ int slots_of(const KvAttention& a, int len) {
-  const int n = (len + a.kv.block - 1) / a.kv.block;
-  return a.blocks != nullptr && a.blocks_width < n ? a.blocks_width : n;
-}
-
-__device__ __forceinline__ uint32_t tiles_of(const KvAttention& a, int len) {
-  return static_cast<uint32_t>((static_cast<long long>(slots_of(a, len)) * a.kv.block + kTile - 1) / kTile);
+// Tiles of the blocks of a request that are read: all that hold tokens, or the
+// listed ones.
+__device__ __forceinline__ uint32_t tiles_of(const KvAttention& a, const Work& w, int len) {
+  const int n = w.by_block.quotient(len + a.kv.block - 1);
+  const uint32_t slots = a.blocks != nullptr && a.blocks_width < n ? a.blocks_width : n;
+  return (slots * a.kv.block + kTile - 1) / kTile;
 }
 
 // first[b] of every request and of their end, and the requests' lengths, by the
 // whole CTA.
-__device__ __forceinline__ void first_tiles(const KvAttention& a, uint32_t* first, int* lens, uint32_t* scratch) {
+__device__ __forceinline__ void first_tiles(const KvAttention& a, const Work& w, uint32_t* first, int* lens, uint32_t* scratch) {
   const int n = a.req.requests, per = (n + blockDim.x - 1) / blockDim.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int b0 = min(n, static_cast<int>(threadIdx.x) * per), b1 = min(n, b0 + per);
   uint32_t mine = 0;
@@ -169,7 +169,7 @@ __device__ __forceinline__ void first_tiles(const KvAttention& a, uint32_t* firs
     const int len = length_of(a, b);
     lens[b] = len;
     first[b] = mine;
-    mine += tiles_of(a, len);
+    mine += tiles_of(a, w, len);
   }
   uint32_t upto = mine;
 #pragma unroll
@@ -180,7 +180,7 @@ __device__ __forceinline__ void first_tiles(const KvAttention& a, uint32_t* firs
   if (lane == 31) scratch[warp] = upto;
   __syncthreads();
   uint32_t before = upto - mine;
-  for (int w = 0; w < warp; ++w) before += scratch[w];
+  for (int i = 0; i < warp; ++i) before += scratch[i];
   for (int b = b0; b < b1; ++b) first[b] += before;
   if (threadIdx.x == blockDim.x - 1) first[n] = before + mine;
   __syncthreads();
@@ -212,12 +212,12 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
   int* lens = reinterpret_cast<int*>(first + a.req.requests + 1);
   const uint32_t warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
-  const int D = a.kv.dim, bs = a.kv.block, G = a.q.heads / a.kv.kv_heads, n = a.req.requests;
+  const int D = a.kv.dim, bs = a.kv.block, G = w.shared, n = a.req.requests;
   launch_dependents();
   if (D < DP)  // what the copies leave of a row stays zero
     for (int i = threadIdx.x; i < S::kRingBytes / 16; i += blockDim.x)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-  first_tiles(a, first, lens, scratch);
+  first_tiles(a, w, first, lens, scratch);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= n; i += blockDim.x) w.first[i] = first[i];
   for (int b = blockIdx.x; b < n; b += gridDim.x)  // requests without tokens
@@ -226,7 +226,7 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
         *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + static_cast<long long>(b) * a.q.heads * D + i) = 0u;
       for (int i = threadIdx.x; i < a.q.heads; i += blockDim.x) a.lse[static_cast<long long>(b) * a.q.heads + i] = -INFINITY;
     }
-  const KvPlan plan = KvPlan::make(first[n], w.most_ranges, kLeastTiles);
+  const KvPlan plan = KvPlan::make(first[n], w.by_ranges);
   if (plan.tiles == 0) return;
   const uint32_t units = static_cast<uint32_t>(plan.ranges) * w.groups;
   // few units: one to a CTA before two
@@ -235,8 +235,8 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
   const uint32_t ring = dev::smem_u32(smem) + warp * S::kStages * S::kStageBytes;
 
   for (uint32_t unit = blockIdx.x * per_cta + warp; unit < units; unit += gridDim.x * per_cta) {
-    const int r = static_cast<int>(unit / w.groups), group = static_cast<int>(unit - r * w.groups);
-    const int per_head = (G + kRowGroup - 1) / kRowGroup, g = group / per_head, row0 = group % per_head * kRowGroup;
+    const int r = static_cast<int>(w.by_groups.quotient(unit)), group = static_cast<int>(unit) - r * w.groups;
+    const int g = w.by_groups_each.quotient(group), row0 = (group - g * w.groups_each) * kRowGroup;
     const int rows = min(kRowGroup, G - row0);
     const uint32_t lo = plan.begin(r), hi = plan.begin(r + 1);
     const T* cache = static_cast<const T*>(a.kv.base) + g * a.kv.head_stride;
@@ -264,8 +264,8 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
       v.page = -1;
       if (tile >= hi) return v;
       while (first[v.b + 1] <= tile) ++v.b;
-      const int len = lens[v.b], blocks = (len + bs - 1) / bs;
-      v.slot = static_cast<int>((tile - first[v.b]) * kTile / static_cast<uint32_t>(bs));
+      const int len = lens[v.b], blocks = w.by_block.quotient(len + bs - 1);
+      v.slot = static_cast<int>(w.by_block.quotient((tile - first[v.b]) * kTile));
       int block = v.slot + lane;
       if (a.blocks != nullptr)
         block = block < min(blocks, a.blocks_width)
@@ -289,24 +289,6 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
     for (uint32_t ahead = lo; ahead < hi + (S::kStages - 1); ++ahead) {
       const uint32_t tile = ahead - (S::kStages - 1);  // whose products are taken, if ahead >= lo + kStages - 1
       const bool takes = ahead >= lo + (S::kStages - 1);
-      if (ahead == lo || (takes && tile >= end)) {  // a request's first: its heads' rows
-        while (first[b + 1] <= (takes ? tile : lo)) ++b;
-        end = first[b + 1];
-        const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
-            q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
-                          ? 0u
-                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
-          }
-#pragma unroll
-        for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
-      }
       if (takes) {
         cp_wait<S::kStages - 2>();
         __syncwarp();
@@ -318,7 +300,7 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
         }
         constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
         const uint32_t t = (ahead - first[now.b]) * kTile + (lane & 15);
-        const int slot = static_cast<int>(t / static_cast<uint32_t>(bs)), off = static_cast<int>(t - slot * static_cast<uint32_t>(bs));
+        const int slot = static_cast<int>(w.by_block.quotient(t)), off = static_cast<int>(t) - slot * bs;
         const int page = __shfl_sync(0xffffffffu, now.page, slot - now.slot);
         const bool row_ok = off < __shfl_sync(0xffffffffu, now.tokens, slot - now.slot) && page >= 0 && page < a.kv.pages;
         const long long row_at = row_ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
@@ -340,6 +322,24 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
         into = into + 1 == S::kStages ? 0 : into + 1;
       }
       cp_commit();
+      if (ahead == lo || (takes && tile >= end)) {  // a request's first: its heads' rows
+        while (first[b + 1] <= (takes ? tile : lo)) ++b;
+        end = first[b + 1];
+        const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+            q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
+                          ? 0u
+                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
+          }
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+      }
       if (!takes) continue;
       const uint32_t ok = valid_of[warp][stage];
       const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + kTile * DP * 2;
@@ -485,7 +485,7 @@ __device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, ui
   __shared__ float total[kMassHeads];
   const int b = cta / w.mass_ctas, j = (cta - b * w.mass_ctas) * kMassBlocks + threadIdx.x / 32;
   const int lane = threadIdx.x % 32, H = a.q.heads, per = a.kv.block / kTile;
-  const int G = H / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
+  const int G = w.shared, per_head = w.groups_each;
   wait_for_parent();
   const uint32_t f0 = w.first[b], f1 = w.first[b + 1];  // a request's tiles are all its blocks'
   const int t0 = j * per, blocks = (f1 - f0 + per - 1) / per;
@@ -497,7 +497,7 @@ __device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, ui
 #pragma unroll
   for (int i = 0; i < kMassAhead; ++i) ahead[i] = i * 32 + lane < count ? z[i * 32 + lane] : -INFINITY;
   if (j < blocks) old = *mass;
-  const KvPlan plan = KvPlan::make(w.first[a.req.requests], w.most_ranges, kLeastTiles);
+  const KvPlan plan = KvPlan::make(w.first[a.req.requests], w.by_ranges);
   const int r0 = plan.of(f0), r1 = plan.of(f1 - 1), slot0 = plan.slot(r0, f0);
   for (int h = threadIdx.x / 8; h < (H + 3) / 4 * 4; h += kJoinWarps * 4) {  // whole warps: they shuffle
     float m = -INFINITY, l = 0.f;
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4)
   __shared__ __align__(16) float sum_o[kJoinWarps][kColumns];
   __shared__ float sum_m[kJoinWarps], sum_l[kJoinWarps];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps_each = kJoinWarps / units_each, mine = warp % warps_each;
-  const int D = a.kv.dim, G = a.q.heads / a.kv.kv_heads, per_head = (G + kRowGroup - 1) / kRowGroup;
+  const int D = a.kv.dim, G = w.shared, per_head = w.groups_each;
   const int chunks = (D + kColumns - 1) / kColumns, unit = (blockIdx.x - item * j.ctas_each) * units_each + warp / warps_each;
   const int h = unit / chunks, d = unit % chunks * kColumns + lane % LANES * 4;
   const bool on = h < a.q.heads && d < D;
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4)
   wait_for_parent();
   const uint32_t tiles = w.first[a.req.requests];
   if (tiles == 0) return;
-  const KvPlan plan = KvPlan::make(tiles, w.most_ranges, kLeastTiles);
+  const KvPlan plan = KvPlan::make(tiles, w.by_ranges);
   int b = item;
   if (by_cut) {
     if (b + 1 >= plan.ranges) return;
@@ -654,9 +654,15 @@ uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
 uint64_t lay_out(int requests, int width, int block, int heads, int kv_heads, int dim, bool mass, int sms, void* base,
                  Work& w) {
   const int G = heads / kv_heads, warps = sms * (padded(dim) == 256 ? Shape<256>::kWarps : Shape<128>::kWarps);
-  w.groups = kv_heads * ((G + kRowGroup - 1) / kRowGroup);
+  w.shared = G;
+  w.groups_each = (G + kRowGroup - 1) / kRowGroup;
+  w.groups = kv_heads * w.groups_each;
   w.rows = G <= 8 ? 8 : 16;
   w.most_ranges = warps / w.groups > 0 ? warps / w.groups : 1;
+  w.by_ranges = FastDiv::make(w.most_ranges);
+  w.by_block = FastDiv::make(block);
+  w.by_groups = FastDiv::make(w.groups);
+  w.by_groups_each = FastDiv::make(w.groups_each);
   w.max_tiles = static_cast<int>((static_cast<int64_t>(width) * block + kTile - 1) / kTile);
   w.mass_ctas = mass ? (width + kMassBlocks - 1) / kMassBlocks : 0;
   const uint64_t parts = 2ull * w.most_ranges * w.groups * w.rows;

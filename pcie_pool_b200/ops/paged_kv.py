@@ -88,8 +88,8 @@ def _requests(torch, block_table, context_lens, device: int, block: int):
         raise ValueError(f"at most {MAX_BLOCK} tokens a block")
     if width * block > 2**31 - 2 * MAX_BLOCK:
         raise ValueError("block_table is too wide: a request has at most 2**31 tokens")
-    if n * width * block >= 2**35:
-        raise ValueError("block_table is too large: at most 2**35 tokens in all")
+    if n * width * block >= 2**34:
+        raise ValueError("block_table is too large: at most 2**34 tokens in all")
     if col != 1 and width > 1:
         raise ValueError("block_table's rows must be contiguous")
     if n > 1 and not context_lens.is_contiguous():

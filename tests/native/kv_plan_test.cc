@@ -9,6 +9,7 @@
 
 #include "kv_plan.h"
 
+using ppb::FastDiv;
 using ppb::KvPlan;
 
 #define CHECK(x)                                                     \
@@ -19,12 +20,13 @@ using ppb::KvPlan;
     }                                                                \
   } while (0)
 
-static void check(const std::vector<uint32_t>& tiles, int most, int least) {
+static void check(const std::vector<uint32_t>& tiles, int most) {
   std::vector<uint32_t> first{0};
   for (uint32_t t : tiles) first.push_back(first.back() + t);
-  const KvPlan p = KvPlan::make(first.back(), most, least);
-  CHECK(p.ranges >= 1 && p.ranges <= most);
+  const KvPlan p = KvPlan::make(first.back(), FastDiv::make(most));
+  CHECK(p.ranges <= most);
   if (p.tiles == 0) return;
+  CHECK(p.ranges >= 1);
   CHECK(p.begin(0) == 0 && p.begin(p.ranges) == p.tiles);
   std::set<std::pair<size_t, int>> written;  // (request, slot)
   std::set<int> slots;
@@ -57,12 +59,18 @@ int main() {
   for (int i = 0; i < 4000; ++i) {
     std::vector<uint32_t> t(1 + rng() % (i % 4 ? 20 : 900));
     for (auto& v : t) v = rng() % 3 == 0 ? 0 : 1 + rng() % (1 << rng() % 14);
-    check(t, 1 + static_cast<int>(rng() % 1200), 1 + static_cast<int>(rng() % 4));
+    check(t, 1 + static_cast<int>(rng() % 1200));
   }
-  check({1u << 31}, 1184, 2);
-  check({1, (1u << 31) - 2, 1}, 1184, 2);
-  check({(1u << 31) - 1}, 32767, 1);
-  check({0, 0, 1, 0}, 148, 2);
-  check({0}, 148, 2);
+  check({(1u << 31) - 1}, 1184);
+  check({1, (1u << 31) - 3, 1}, 1184);
+  check({(1u << 31) - 1}, 32767);
+  for (int i = 0; i < 2000000; ++i) {
+    const uint32_t d = 1 + rng() % (i % 3 ? 70000u : 0x7fffffffu), n = rng() % 0x80000000u;
+    const FastDiv f = FastDiv::make(d);
+    CHECK(f.quotient(n) == n / d && f.quotient(n / d * d) == n / d && (n < d || f.quotient(n / d * d - 1) == n / d - 1));
+    CHECK(f.quotient(0x7fffffffu) == 0x7fffffffu / d);
+  }
+  check({0, 0, 1, 0}, 148);
+  check({0}, 148);
   std::printf("kv_plan_test: ok\n");
 }
