@@ -54,8 +54,8 @@ struct Shape {
 struct Work {
   float* part_o;        // [2 ranges, groups, rows, dim]
   float2* part_ml;      // [2 ranges, groups, rows]: maximum (base 2) and sum
-  uint32_t* first;      // [requests + 1]
-  int* begins;          // [ranges]: the request of a range's first tile
+  int4* items;          // what there may be to join, by request or by cut: request, ranges, first slot
+  uint32_t* first;      // [requests + 1], for the mass
   float* z;             // [requests, max_tiles, heads]: log2 of a tile's sum, or null
   int max_tiles;        // of a request
   int mass_ctas;        // of a request
@@ -63,6 +63,7 @@ struct Work {
   int shared;           // query heads of a key head
   int groups_each;      // row groups of a key head
   int groups;           // of all key heads
+  bool by_cut;          // more requests than cuts: items go by cut
   FastDiv by_ranges, by_block, by_groups, by_groups_each;
   int rows;             // of a group's partial result: 8 or 16
 };
@@ -199,6 +200,36 @@ __device__ __forceinline__ int request_of(const uint32_t* first, int n, uint32_t
   return lo;
 }
 
+// What the kernels behind need to know, and the results of requests without tokens;
+// the warps of all CTAs take the requests (or the cuts) in turn.
+template <typename T>
+__device__ __forceinline__ void note_items(const KvAttention& a, const Work& w, const uint32_t* first, const KvPlan& plan) {
+  const int lane = threadIdx.x % 32, n = a.req.requests;
+  const int warp = threadIdx.x / 32 * gridDim.x + blockIdx.x, warps = gridDim.x * (blockDim.x / 32);
+  for (int b = warp; b < n; b += warps) {
+    if (w.z != nullptr && lane == 0) w.first[b] = first[b];
+    if (first[b] == first[b + 1]) {
+      T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.q.heads * a.kv.dim;
+      for (int i = 2 * lane; i < a.q.heads * a.kv.dim; i += 64) *reinterpret_cast<uint32_t*>(out + i) = 0u;
+      for (int i = lane; i < a.q.heads; i += 32) a.lse[static_cast<long long>(b) * a.q.heads + i] = -INFINITY;
+    }
+  }
+  if (w.z != nullptr && warp == 0 && lane == 0) w.first[n] = first[n];
+  const int items = w.by_cut ? w.most_ranges - 1 : n;
+  for (int i = warp + lane * warps; i < items; i += warps * 32) {
+    int4 v = make_int4(0, 0, 0, 0);  // nothing to join
+    v.x = w.by_cut ? i + 1 < plan.ranges ? request_of(first, n, plan.begin(i + 1)) : -1 : i;
+    if (v.x >= 0 && first[v.x] < first[v.x + 1]) {
+      v.y = plan.of(first[v.x]);
+      v.z = plan.of(first[v.x + 1] - 1);
+      // the first part may lie in its range's second place, the others lie in the first
+      v.w = plan.slot(v.y, first[v.x]);
+      if (w.by_cut && v.y != i) v.z = v.y;  // not its request's first cut
+    }
+    w.items[i] = v;
+  }
+}
+
 // DP: dim padded to 64, 128 or 256.  PACKED: at most eight heads share a key head,
 // rows 8 to 15 carry the weights' remainders.
 template <typename T, int DP, bool PACKED>
@@ -218,23 +249,18 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
     for (int i = threadIdx.x; i < S::kRingBytes / 16; i += blockDim.x)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   first_tiles(a, w, first, lens, scratch);
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= n; i += blockDim.x) w.first[i] = first[i];
-  for (int b = blockIdx.x; b < n; b += gridDim.x)  // requests without tokens
-    if (first[b] == first[b + 1]) {
-      for (int i = 2 * threadIdx.x; i < a.q.heads * D; i += 2 * blockDim.x)
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + static_cast<long long>(b) * a.q.heads * D + i) = 0u;
-      for (int i = threadIdx.x; i < a.q.heads; i += blockDim.x) a.lse[static_cast<long long>(b) * a.q.heads + i] = -INFINITY;
-    }
   const KvPlan plan = KvPlan::make(first[n], w.by_ranges);
-  if (plan.tiles == 0) return;
   const uint32_t units = static_cast<uint32_t>(plan.ranges) * w.groups;
   // few units: one to a CTA before two
   const uint32_t per_cta = min(static_cast<uint32_t>(S::kWarps), (units + gridDim.x - 1) / gridDim.x);
-  if (warp >= per_cta) return;
+  const uint32_t unit0 = blockIdx.x * per_cta + warp;
+  if (warp >= per_cta || unit0 >= units) {
+    note_items<T>(a, w, first, plan);
+    return;
+  }
   const uint32_t ring = dev::smem_u32(smem) + warp * S::kStages * S::kStageBytes;
 
-  for (uint32_t unit = blockIdx.x * per_cta + warp; unit < units; unit += gridDim.x * per_cta) {
+  for (uint32_t unit = unit0; unit < units; unit += gridDim.x * per_cta) {
     const int r = static_cast<int>(w.by_groups.quotient(unit)), group = static_cast<int>(unit) - r * w.groups;
     const int g = w.by_groups_each.quotient(group), row0 = (group - g * w.groups_each) * kRowGroup;
     const int rows = min(kRowGroup, G - row0);
@@ -245,7 +271,6 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
     uint32_t q[DP / 16][4];
     const float to_base2 = a.scale * kLog2e;
     int b = request_of(first, n, lo);
-    if (group == 0 && lane == 0) w.begins[r] = b;
     uint32_t end = 0;  // of request b's tiles
 
     // A window is 32 neighbouring blocks of a request, a lane each: their pages, and
@@ -280,6 +305,10 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
       return v;
     };
     Window next = look_up(lo, b), now = next;
+    if (unit == unit0) {  // while the first blocks are looked up
+      note_items<T>(a, w, first, plan);
+      __syncwarp();
+    }
     now.end = lo;
 
     // The copies run kStages - 1 tiles ahead of the products.  One loop does both, so
@@ -471,7 +500,6 @@ struct Join {
   uint32_t ctas;       // that join; the others add the mass
   uint32_t ctas_each;  // of a request, or of a cut
   int units_each;
-  bool by_cut;
 };
 
 // The mass of kMassBlocks blocks of a request, a warp for each: the sums of its
@@ -549,7 +577,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4)
     return;
   }
   const int units_each = j.units_each, item = blockIdx.x / j.ctas_each;
-  const bool by_cut = j.by_cut;
   constexpr int kColumns = 4 * LANES, kAtOnce = 32 / LANES;
   __shared__ __align__(16) float sum_o[kJoinWarps][kColumns];
   __shared__ float sum_m[kJoinWarps], sum_l[kJoinWarps];
@@ -562,19 +589,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4)
   const long long base = static_cast<long long>(h / G * per_head + h % G / kRowGroup) * w.rows + h % G % kRowGroup;
   const long long step = static_cast<long long>(w.groups) * w.rows;
   wait_for_parent();
-  const uint32_t tiles = w.first[a.req.requests];
-  if (tiles == 0) return;
-  const KvPlan plan = KvPlan::make(tiles, w.by_ranges);
-  int b = item;
-  if (by_cut) {
-    if (b + 1 >= plan.ranges) return;
-    b = w.begins[b + 1];
-  }
-  const uint32_t f0 = w.first[b], f1 = w.first[b + 1];
-  if (f0 == f1) return;
-  const int r0 = plan.of(f0), r1 = plan.of(f1 - 1);
-  if (r0 == r1 || (by_cut && r0 != item)) return;  // finished where it was computed
-  const int slot0 = plan.slot(r0, f0);  // the first part may lie in its range's second place, the others lie in the first
+  const int4 found = w.items[item];
+  const int b = found.x, r0 = found.y, r1 = found.z, slot0 = found.w;
+  if (r0 == r1) return;  // finished where it was computed
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   int r = r0 + mine * kAtOnce * kJoinParts + lane / LANES;
@@ -674,8 +691,9 @@ uint64_t lay_out(int requests, int width, int block, int heads, int kv_heads, in
   at += up(parts * 8);
   w.first = reinterpret_cast<uint32_t*>(p + at);
   at += up((requests + 1ull) * 4);
-  w.begins = reinterpret_cast<int*>(p + at);
-  at += up(w.most_ranges * 4ull);
+  w.by_cut = requests >= w.most_ranges;
+  w.items = reinterpret_cast<int4*>(p + at);
+  at += up((w.by_cut ? w.most_ranges : requests) * 16ull);
   w.z = mass ? reinterpret_cast<float*>(p + at) : nullptr;
   if (mass) at += up(uint64_t(requests) * w.max_tiles * heads * 4);
   return at;
@@ -720,8 +738,7 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
   rc = cudaGetLastError();
   if (rc != cudaSuccess) return rc;
   Join j;
-  j.by_cut = a.req.requests >= w.most_ranges;
-  const uint32_t items = j.by_cut ? w.most_ranges - 1 : a.req.requests;
+  const uint32_t items = w.by_cut ? w.most_ranges - 1 : a.req.requests;
   // narrow units while the CTAs fit beside the attention's, else whole rows, and
   // as many warps for a unit as leave two CTAs to an SM
   auto join = w.z ? attention_join_kernel<T, 8, true> : attention_join_kernel<T, 8, false>;
