@@ -311,46 +311,28 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
     }
     now.end = lo;
 
-    // The copies run kStages - 1 tiles ahead of the products.  One loop does both, so
-    // that no code stands twice: at the start of a kernel instructions come from
-    // memory too, and wait in line with the first tiles.
-    int stage = 0, into = 0;
-    for (uint32_t ahead = lo; ahead < hi + (S::kStages - 1); ++ahead) {
-      const uint32_t tile = ahead - (S::kStages - 1);  // whose products are taken, if ahead >= lo + kStages - 1
-      const bool takes = ahead >= lo + (S::kStages - 1);
-      if (takes) {
-        cp_wait<S::kStages - 2>();
-        __syncwarp();
-      }
-      if (ahead < hi) {  // into the stage that the last step emptied
-        if (ahead >= now.end) {
-          now = next;
-          next = look_up(now.end, now.b);
-        }
-        constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
-        const uint32_t t = (ahead - first[now.b]) * kTile + (lane & 15);
-        const int slot = static_cast<int>(w.by_block.quotient(t)), off = static_cast<int>(t) - slot * bs;
-        const int page = __shfl_sync(0xffffffffu, now.page, slot - now.slot);
-        const bool row_ok = off < __shfl_sync(0xffffffffu, now.tokens, slot - now.slot) && page >= 0 && page < a.kv.pages;
-        const long long row_at = row_ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
-        const uint32_t ok = __ballot_sync(0xffffffffu, row_ok) & 0xffffu;
-        if (lane == 0) valid_of[warp][into] = ok;
-        const uint32_t to = ring + into * S::kStageBytes;
+    // Keys and values have rings of kStages tiles each: the keys of a tile are asked
+    // for kStages tiles ahead, its values kStages - 1, each as soon as its place has
+    // been read, so that 2 kStages - 1 of the 2 kStages places are always on their way.
+    // One loop does copies and products, so that no code stands twice: at the
+    // start of a kernel instructions come from memory too, and wait in line with the
+    // first tiles.
+    constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
+    long long row_at = 0;  // where lane & 15's row of the tile asked for last begins
+    uint32_t rows_ok = 0;
+    auto copy = [&](uint32_t to, long long from) {
 #pragma unroll
-        for (int i = 0; i < kTile * kChunks / 32; ++i) {
-          const int row = (i * 32 + lane) / kChunks, chunk = (i * 32 + lane) % kChunks;
-          const long long at = __shfl_sync(0xffffffffu, row_at, row) + chunk * 8;
-          const uint32_t dst = to + row * DP * 2 + ((chunk ^ (row & 7)) * 16);
-          if (chunk * 8 < D) {
-            const T* src = cache + at;
-            const bool v = ok >> row & 1;
-            cp_async16(dst, v ? src : a.kv.base, v);
-            cp_async16(dst + kTile * DP * 2, v ? src + a.kv.lane_stride : a.kv.base, v);
-          }
-        }
-        into = into + 1 == S::kStages ? 0 : into + 1;
+      for (int i = 0; i < kTile * kChunks / 32; ++i) {
+        const int row = (i * 32 + lane) / kChunks, chunk = (i * 32 + lane) % kChunks;
+        const T* src = cache + from + __shfl_sync(0xffffffffu, row_at, row) + chunk * 8;
+        const bool ok = rows_ok >> row & 1;
+        if (chunk * 8 < D) cp_async16(to + row * DP * 2 + ((chunk ^ (row & 7)) * 16), ok ? src : a.kv.base, ok);
       }
-      cp_commit();
+    };
+    int stage = 0, into = 0;  // places of `tile` and `ahead`
+    for (uint32_t ahead = lo; ahead < hi + S::kStages; ++ahead) {
+      const uint32_t tile = ahead - S::kStages;  // whose products are taken, if ahead >= lo + kStages
+      const bool takes = ahead >= lo + S::kStages;
       if (ahead == lo || (takes && tile >= end)) {  // a request's first: its heads' rows
         while (first[b + 1] <= (takes ? tile : lo)) ++b;
         end = first[b + 1];
@@ -369,75 +351,103 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.f;
       }
-      if (!takes) continue;
-      const uint32_t ok = valid_of[warp][stage];
-      const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + kTile * DP * 2;
+      if (takes) {
+        cp_wait<2 * S::kStages - 2>();  // the tile's keys
+        __syncwarp();
+      }
+      // the values of the tile whose keys were asked for in the last step, into the
+      // place that the last step's products emptied
+      if (ahead > lo && ahead <= hi) copy(ring + (into == 0 ? S::kStages - 1 : into - 1) * S::kStageBytes + kTile * DP * 2, a.kv.lane_stride);
+      cp_commit();
       float s[2][4] = {};
-      {
-        const int row = (lane & 7) + ((lane >> 4) << 3);
-        const uint32_t base = ks + row * DP * 2;
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          uint32_t f[4];
-          ldsm4(f, base + (((2 * k + ((lane >> 3) & 1)) ^ (row & 7)) * 16));
-          Type<T>::mma(s[0], q[k], f[0], f[1]);
-          Type<T>::mma(s[1], q[k], f[2], f[3]);
-        }
-      }
       constexpr int kHalves = PACKED ? 1 : 2;  // row lane / 4, and the one eight below
-      bool grew = false;
-      float ratio[2];
-#pragma unroll
-      for (int x = 0; x < kHalves; ++x) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = (lane & 3) * 2 + (i & 1) + (i >> 1) * 8;
-          float& v = s[i >> 1][2 * x + (i & 1)];
-          v = ok >> col & 1 ? v * to_base2 : -INFINITY;
-          top = fmaxf(top, v);
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float now = fmaxf(m[x], top), at = now == -INFINITY ? 0.f : now;
-        ratio[x] = ex2(m[x] - at);
-        grew |= now > m[x];
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float& v = s[i >> 1][2 * x + (i & 1)];
-          v = ex2(v - at);
-          sum += v;
-        }
-        m[x] = now;
-        l[x] = l[x] * ratio[x] + sum;  // of this lane's columns
-        if (w.z != nullptr) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          const int row = lane / 4 + 8 * x;
-          if ((lane & 3) == 0 && row < rows)
-            w.z[(static_cast<long long>(b) * w.max_tiles + (tile - first[b])) * a.q.heads + g * G + row0 + row] = at + lg2(sum);
-        }
-      }
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
-          o[i][0] *= ratio[0];
-          o[i][1] *= ratio[0];
-          o[i][2] *= ratio[kHalves - 1];
-          o[i][3] *= ratio[kHalves - 1];
-        }
-      }
       uint32_t p[4], rest[4];
-      if constexpr (PACKED) {
-        split<T>(s[0][0], s[0][1], p[0], p[1]);
-        split<T>(s[1][0], s[1][1], p[2], p[3]);
-      } else {
-        split<T>(s[0][0], s[0][1], p[0], rest[0]);
-        split<T>(s[0][2], s[0][3], p[1], rest[1]);
-        split<T>(s[1][0], s[1][1], p[2], rest[2]);
-        split<T>(s[1][2], s[1][3], p[3], rest[3]);
+      if (takes) {
+        const uint32_t ok = valid_of[warp][stage];
+        const uint32_t ks = ring + stage * S::kStageBytes;
+        {
+          const int row = (lane & 7) + ((lane >> 4) << 3);
+          const uint32_t base = ks + row * DP * 2;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            uint32_t f[4];
+            ldsm4(f, base + (((2 * k + ((lane >> 3) & 1)) ^ (row & 7)) * 16));
+            Type<T>::mma(s[0], q[k], f[0], f[1]);
+            Type<T>::mma(s[1], q[k], f[2], f[3]);
+          }
+        }
+        bool grew = false;
+        float ratio[2];
+#pragma unroll
+        for (int x = 0; x < kHalves; ++x) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int col = (lane & 3) * 2 + (i & 1) + (i >> 1) * 8;
+            float& v = s[i >> 1][2 * x + (i & 1)];
+            v = ok >> col & 1 ? v * to_base2 : -INFINITY;
+            top = fmaxf(top, v);
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float now = fmaxf(m[x], top), at = now == -INFINITY ? 0.f : now;
+          ratio[x] = ex2(m[x] - at);
+          grew |= now > m[x];
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& v = s[i >> 1][2 * x + (i & 1)];
+            v = ex2(v - at);
+            sum += v;
+          }
+          m[x] = now;
+          l[x] = l[x] * ratio[x] + sum;  // of this lane's columns
+          if (w.z != nullptr) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int row = lane / 4 + 8 * x;
+            if ((lane & 3) == 0 && row < rows)
+              w.z[(static_cast<long long>(b) * w.max_tiles + (tile - first[b])) * a.q.heads + g * G + row0 + row] = at + lg2(sum);
+          }
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            o[i][0] *= ratio[0];
+            o[i][1] *= ratio[0];
+            o[i][2] *= ratio[kHalves - 1];
+            o[i][3] *= ratio[kHalves - 1];
+          }
+        }
+        if constexpr (PACKED) {
+          split<T>(s[0][0], s[0][1], p[0], p[1]);
+          split<T>(s[1][0], s[1][1], p[2], p[3]);
+        } else {
+          split<T>(s[0][0], s[0][1], p[0], rest[0]);
+          split<T>(s[0][2], s[0][3], p[1], rest[1]);
+          split<T>(s[1][0], s[1][1], p[2], rest[2]);
+          split<T>(s[1][2], s[1][3], p[3], rest[3]);
+        }
+        cp_wait<2 * S::kStages - 2>();  // its values
+        __syncwarp();
       }
+      if (ahead < hi) {  // the keys of the tile kStages ahead, into the place of this one's
+        const bool entered = ahead >= now.end;  // the next window
+        if (entered) now = next;
+        const uint32_t t = (ahead - first[now.b]) * kTile + (lane & 15);
+        const int slot = static_cast<int>(w.by_block.quotient(t)), off = static_cast<int>(t) - slot * bs;
+        const int page = __shfl_sync(0xffffffffu, now.page, slot - now.slot);
+        const bool ok = off < __shfl_sync(0xffffffffu, now.tokens, slot - now.slot) && page >= 0 && page < a.kv.pages;
+        row_at = ok ? page * a.kv.page_stride + off * a.kv.token_stride : 0;
+        rows_ok = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+        if (lane == 0) valid_of[warp][into] = rows_ok;
+        copy(ring + into * S::kStageBytes, 0);
+        if (entered) next = look_up(now.end, now.b);
+      }
+      cp_commit();
+      into = into + 1 == S::kStages ? 0 : into + 1;
+      if (!takes) continue;
+      const uint32_t vs = ring + stage * S::kStageBytes + kTile * DP * 2;
       {
         const int row = lane & 15;
         const uint32_t base = vs + row * DP * 2;
