@@ -231,8 +231,8 @@ __device__ __forceinline__ void note_items(const KvAttention& a, const Work& w, 
 }
 
 // DP: dim padded to 64, 128 or 256.  PACKED: at most eight heads share a key head,
-// rows 8 to 15 carry the weights' remainders.
-template <typename T, int DP, bool PACKED>
+// rows 8 to 15 carry the weights' remainders.  MASS: the tiles' sums are kept.
+template <typename T, int DP, bool PACKED, bool MASS>
 __global__ void __maxnreg__(Shape<DP>::kRegisters)
     attention_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w) {
   using S = Shape<DP>;
@@ -402,7 +402,7 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
           }
           m[x] = now;
           l[x] = l[x] * ratio[x] + sum;  // of this lane's columns
-          if (w.z != nullptr) {
+          if (MASS) {
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             const int row = lane / 4 + 8 * x;
@@ -442,7 +442,13 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
         rows_ok = __ballot_sync(0xffffffffu, ok) & 0xffffu;
         if (lane == 0) valid_of[warp][into] = rows_ok;
         copy(ring + into * S::kStageBytes, 0);
-        if (entered) next = look_up(now.end, now.b);
+        if (entered) {
+          const int d = lane * 64;  // of its heads' rows, 128 bytes a lane
+          if (d < rows * D)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const T*>(a.q.base) + now.b * a.q.stride +
+                                                          (g * G + row0 + d / D) * a.q.head_stride + d % D));
+          next = look_up(now.end, now.b);
+        }
       }
       cp_commit();
       into = into + 1 == S::kStages ? 0 : into + 1;
@@ -733,16 +739,18 @@ cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, cuda
 template <typename T, int DP>
 cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cudaStream_t stream) {
   const int smem = Shape<DP>::kRingBytes + (2 * a.req.requests + 1) * 4, threads = Shape<DP>::kWarps * 32;
-  auto kernel = w.rows == 8 ? attention_kernel<T, DP, true> : attention_kernel<T, DP, false>;
+  auto kernel = w.rows == 8 ? (w.z ? attention_kernel<T, DP, true, true> : attention_kernel<T, DP, true, false>)
+                            : (w.z ? attention_kernel<T, DP, false, true> : attention_kernel<T, DP, false, false>);
+  const int which = (w.rows == 8) + 2 * (w.z != nullptr);
   static_assert(Shape<DP>::kRingBytes + (2 * kMostRequests + 1) * 4 <= 226 * 1024, "more shared memory than an SM has");
-  static std::atomic<uint64_t> ready[2];  // devices that know the kernels' shared memory
+  static std::atomic<uint64_t> ready[4];  // devices that know the kernels' shared memory
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   cudaError_t rc = cudaSuccess;
-  if (!(ready[w.rows == 8].load(std::memory_order_relaxed) & bit)) {
+  if (!(ready[which].load(std::memory_order_relaxed) & bit)) {
     rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               Shape<DP>::kRingBytes + (2 * kMostRequests + 1) * 4);
     if (rc != cudaSuccess) return rc;
-    ready[w.rows == 8].fetch_or(bit, std::memory_order_relaxed);
+    ready[which].fetch_or(bit, std::memory_order_relaxed);
   }
   kernel<<<sms, threads, smem, stream>>>(a, w);
   rc = cudaGetLastError();
