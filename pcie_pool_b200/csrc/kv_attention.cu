@@ -27,14 +27,16 @@
 #include <cmath>
 
 #include "device_utils.cuh"
+#include "kv_device.cuh"
 #include "kv_plan.h"
 #include "paged_kv.h"
 
 namespace ppb {
 namespace {
 
+using namespace dev;
+
 constexpr int kTile = 16;      // tokens of a step; the mass is gathered by tiles
-constexpr int kMostRequests = 4096;
 constexpr int kRowGroup = 16;  // query heads of one warp at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -68,15 +70,6 @@ struct Work {
   int rows;             // of a group's partial result: 8 or 16
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -99,9 +92,6 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_parent() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 template <typename T>
 struct Type;
 
@@ -147,57 +137,12 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& 
   lo = Type<T>::pack(x - h.x, y - h.y);
 }
 
-__device__ __forceinline__ int length_of(const KvAttention& a, int b) {
-  const long long most = static_cast<long long>(a.req.width) * a.kv.block;
-  return max(0, static_cast<int>(min(static_cast<long long>(a.req.lens[b]), most)));
-}
-
 // Tiles of the blocks of a request that are read: all that hold tokens, or the
 // listed ones.
 __device__ __forceinline__ uint32_t tiles_of(const KvAttention& a, const Work& w, int len) {
   const int n = w.by_block.quotient(len + a.kv.block - 1);
   const uint32_t slots = a.blocks != nullptr && a.blocks_width < n ? a.blocks_width : n;
   return (slots * a.kv.block + kTile - 1) / kTile;
-}
-
-// first[b] of every request and of their end, and the requests' lengths, by the
-// whole CTA.
-__device__ __forceinline__ void first_tiles(const KvAttention& a, const Work& w, uint32_t* first, int* lens, uint32_t* scratch) {
-  const int n = a.req.requests, per = (n + blockDim.x - 1) / blockDim.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int b0 = min(n, static_cast<int>(threadIdx.x) * per), b1 = min(n, b0 + per);
-  uint32_t mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int len = length_of(a, b);
-    lens[b] = len;
-    first[b] = mine;
-    mine += tiles_of(a, w, len);
-  }
-  uint32_t upto = mine;
-#pragma unroll
-  for (int x = 1; x < 32; x *= 2) {
-    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, x);
-    if (lane >= x) upto += v;
-  }
-  if (lane == 31) scratch[warp] = upto;
-  __syncthreads();
-  uint32_t before = upto - mine;
-  for (int i = 0; i < warp; ++i) before += scratch[i];
-  for (int b = b0; b < b1; ++b) first[b] += before;
-  if (threadIdx.x == blockDim.x - 1) first[n] = before + mine;
-  __syncthreads();
-}
-
-// The request of a tile: the last b with first[b] <= tile that has tiles.
-__device__ __forceinline__ int request_of(const uint32_t* first, int n, uint32_t tile) {
-  int lo = 0, hi = n;  // first[lo] <= tile < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (first[mid] <= tile)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
 }
 
 // What the kernels behind need to know, and the results of requests without tokens;
@@ -248,7 +193,7 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
   if (D < DP)  // what the copies leave of a row stays zero
     for (int i = threadIdx.x; i < S::kRingBytes / 16; i += blockDim.x)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-  first_tiles(a, w, first, lens, scratch);
+  running_sums(n, [&](int b) { return tiles_of(a, w, lens[b] = length_of(a.req, bs, b)); }, first, scratch);
   const KvPlan plan = KvPlan::make(first[n], w.by_ranges);
   const uint32_t units = static_cast<uint32_t>(plan.ranges) * w.groups;
   // few units: one to a CTA before two
@@ -258,7 +203,7 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
     note_items<T>(a, w, first, plan);
     return;
   }
-  const uint32_t ring = dev::smem_u32(smem) + warp * S::kStages * S::kStageBytes;
+  const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
 
   for (uint32_t unit = unit0; unit < units; unit += gridDim.x * per_cta) {
     const int r = static_cast<int>(w.by_groups.quotient(unit)), group = static_cast<int>(unit) - r * w.groups;
@@ -575,7 +520,7 @@ __device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, ui
     const float v = z[i];
     if (v != -INFINITY) sum += ex2(v - total[i % H]);
   }
-  sum = dev::warp_sum(sum);
+  sum = warp_sum(sum);
   if (j < blocks && lane == 0) *mass = old + sum;
 }
 
@@ -715,27 +660,6 @@ uint64_t lay_out(int requests, int width, int block, int heads, int kv_heads, in
   return at;
 }
 
-cudaError_t sm_count(int* sms, int* device) {
-  cudaError_t rc = cudaGetDevice(device);
-  return rc != cudaSuccess ? rc : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *device);
-}
-
-// A kernel that may be resident before the one ahead of it in the stream is done
-// (it waits for it itself).
-template <typename... Params, typename... Args>
-cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 template <typename T, int DP>
 cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cudaStream_t stream) {
   const int smem = Shape<DP>::kRingBytes + (2 * a.req.requests + 1) * 4, threads = Shape<DP>::kWarps * 32;
@@ -775,7 +699,7 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
   }
   const uint32_t ctas = j.ctas + static_cast<uint32_t>(a.req.requests) * w.mass_ctas;
   if (ctas == 0) return cudaSuccess;
-  return launch_after(join, dim3(ctas), kJoinWarps * 32, stream, a, w, j);
+  return launch_after(join, ctas, kJoinWarps * 32, stream, a, w, j);
 }
 
 template <typename T>

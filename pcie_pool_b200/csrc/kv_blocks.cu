@@ -4,21 +4,23 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <type_traits>
 
+#include "device_utils.cuh"
+#include "kv_device.cuh"
+#include "kv_plan.h"
 #include "paged_kv.h"
 
 namespace ppb {
 namespace {
 
+using namespace dev;
+
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-
-__device__ __forceinline__ int length_of(const KvRequests& r, int block, int b) {
-  return max(0, (int)min((long long)r.lens[b], (long long)r.width * block));
-}
 
 template <typename T>
 struct Pair;
@@ -49,9 +51,6 @@ __device__ __forceinline__ float2 floats(uint32_t v) {
   const T* p = reinterpret_cast<const T*>(&v);
   return make_float2(to_f(p[0]), to_f(p[1]));
 }
-
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_parent() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- key bounds -------------------------------------------------------------------
 // A CTA for each block: a thread takes 8 channels of all its tokens, 16 bytes a load,
@@ -87,9 +86,11 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Pag
 // so a group costs as much as one head.  The sums are taken in 64 bits: products of
 // two 8- or 11-bit numbers and their sums are then exact for all but far-flung
 // exponents, and the order of blocks does not hang on the order of summation.  A
-// warp takes eight blocks of one key head at a time (their loads are in flight
-// together, and their sums are reduced together); it reads `kReach` channels of
-// lower and upper bounds with 8 bytes a lane each.
+// warp takes eight blocks of one key head as a unit, whose sums are reduced together,
+// with 4 of `kReach` channels of a row to a lane.  It asks for all its units' rows
+// before it looks at the first (cp.async, through shared memory, since registers would hold
+// too few): 192 KiB an SM on their way, of a call that fits in one wave all there is.
+// Eight rows at a time in registers took 15 us for 8192 blocks of 8 key heads, 34 MB.
 //
 // The conversion to 64 bits (a sixteenth of the rate of a product) is left out:
 // the bits of a bf16 or fp16 value, moved to where a double keeps its exponent and
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Pag
 // A and B carry half of that power, and the sum gets the other half back.  Infinities
 // and values that are not a number do not move so; a row that has one (0 * x tells)
 // is summed again with converted values.
-constexpr int kScoreWarps = 8, kScoreBlocks = 16, kTogether = 8, kReach = 128;
+constexpr int kScoreWarps = 8, kTogether = 8, kReach = 128;
 
 template <typename T>
 struct Moved;
@@ -126,130 +127,161 @@ __device__ __forceinline__ uint32_t zero_unless_special(uint32_t pair, uint32_t 
   return reinterpret_cast<uint32_t&>(r);
 }
 
-template <typename T, int PARTS>  // PARTS: dim / kReach, rounded up
-__global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_constant__ KvSelect s) {
-  const int b = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32, G = s.q.heads / s.kv_heads;
+// PARTS: dim / kReach, rounded up.  A warp has two units, or one of the longer rows.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_constant__ KvSelect s, FastDiv by_block, FastDiv by_heads) {
+  constexpr int kUnits = 2 / PARTS, kRowBytes = PARTS * kReach * 4;
+  extern __shared__ __align__(128) uint8_t rows[];
+  __shared__ uint32_t scratch[kScoreWarps];
+  uint32_t* starts = reinterpret_cast<uint32_t*>(rows + kScoreWarps * kUnits * kTogether * kRowBytes);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, G = s.q.heads / s.kv_heads;
+  const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(rows)) + warp * kUnits * kTogether * kRowBytes;
+  const int chunks = s.dim / 4;  // 16-byte pieces of a row, both bounds
+  const long long row_bytes = static_cast<long long>(s.kv_heads) * 4 * s.dim;
   launch_dependents();
-  const int from = blockIdx.x * kScoreBlocks;
-  const int* table = s.req.table + b * s.req.table_stride;
-  const int len = s.req.lens[b];
-  // looked up before the length is known, so that the two loads wait together
-  int pages = lane < kScoreBlocks && from + lane < s.req.width ? table[from + lane] : -1;
-  const int n = static_cast<int>((max(0ll, min(static_cast<long long>(len), static_cast<long long>(s.req.width) * s.block)) +
-                                  s.block - 1) / s.block);
-  if (from >= n) return;
-  if (from + lane >= n || pages >= s.pages) pages = -1;
-  const int batches = (min(kScoreBlocks, n - from) + kTogether - 1) / kTogether;
-  double above[PARTS][4], below[PARTS][4];
-  uint32_t above_on[PARTS][2], below_on[PARTS][2];  // channels that count: 0 * inf shall be nothing
-  const int row_values = s.kv_heads * 2 * s.dim;
-  int have = -1;
-  for (int unit = warp; unit < s.kv_heads * batches; unit += kScoreWarps) {
-    const int g = unit % s.kv_heads, first = unit / s.kv_heads * kTogether, j0 = from + first;
-    const T* bounds = static_cast<const T*>(s.bounds) + g * 2 * s.dim + lane * 4;
-    uint2 lo[kTogether][PARTS], hi[kTogether][PARTS];
+  // items are 16 units (8 of longer rows) of a request, of all requests in a row
+  running_sums(s.req.requests,
+               [&](int b) {
+                 const int batches = (by_block.quotient(length_of(s.req, s.block, b) + s.block - 1) + kTogether - 1) / kTogether;
+                 return (batches * s.kv_heads + kScoreWarps * kUnits - 1) / (kScoreWarps * kUnits);
+               },
+               starts, scratch);
+  for (uint32_t item = blockIdx.x; item < starts[s.req.requests]; item += gridDim.x) {
+    const int b = request_of(starts, s.req.requests, item);
+    const uint32_t unit0 = (item - starts[b]) * (kScoreWarps * kUnits) + warp;
+    const int* table = s.req.table + b * s.req.table_stride;
+    const int n = by_block.quotient(length_of(s.req, s.block, b) + s.block - 1);
+    int pages[kUnits], heads[kUnits], first[kUnits];
 #pragma unroll
-    for (int i = 0; i < kTogether; ++i) {
-      const int page = __shfl_sync(0xffffffffu, pages, first + i);
-      const bool there = page >= 0;
-      const T* row = bounds + static_cast<long long>(page) * row_values;
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) {
-        lo[i][p] = hi[i][p] = make_uint2(0, 0);
-        if (there && p * kReach + lane * 4 < s.dim) {
-          lo[i][p] = *reinterpret_cast<const uint2*>(row + p * kReach);
-          hi[i][p] = *reinterpret_cast<const uint2*>(row + s.dim + p * kReach);
-        }
-      }
+    for (int u = 0; u < kUnits; ++u) {
+      const uint32_t unit = unit0 + u * kScoreWarps, batch = by_heads.quotient(unit);
+      heads[u] = unit - batch * s.kv_heads;
+      first[u] = batch * kTogether;
+      pages[u] = lane < kTogether && first[u] + lane < n ? table[first[u] + lane] : -1;
     }
-    if (have != g) {
-      have = g;
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) {
-        double up[4] = {}, down[4] = {};
-        const int d = p * kReach + lane * 4;
-        if (d < s.dim) {
-          const T* q = static_cast<const T*>(s.q.base) + b * s.q.stride + g * G * s.q.head_stride + d;
+    for (int u = 0; u < kUnits; ++u) {
+      if (pages[u] >= s.pages) pages[u] = -1;
+      const uint8_t* from = static_cast<const uint8_t*>(s.bounds) + static_cast<long long>(heads[u]) * 4 * s.dim + lane * 16;
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        const int page = __shfl_sync(0xffffffffu, pages[u], i);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+          if (page >= 0 && p * 32 + lane < chunks)
+            cp_async16(mine + (u * kTogether + i) * kRowBytes + (p * 32 + lane) * 16, from + page * row_bytes + p * 512, true);
+      }
+      cp_commit();
+    }
+    double above[PARTS][4], below[PARTS][4];
+    uint32_t above_on[PARTS][2], below_on[PARTS][2];  // channels that count: 0 * inf shall be nothing
+    int have = -1;
+#pragma unroll 1
+    for (int u = 0; u < kUnits; ++u) {
+      const int g = u ? heads[kUnits - 1] : heads[0], j0 = u ? first[kUnits - 1] : first[0];
+      if (j0 >= n) break;
+      if (have != g) {
+        have = g;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          double up[4] = {}, down[4] = {};
+          const int d = p * kReach + lane * 4;
+          if (d < s.dim) {
+            const T* q = static_cast<const T*>(s.q.base) + b * s.q.stride + g * G * s.q.head_stride + d;
 #pragma unroll 4
-          for (int h = 0; h < G; ++h, q += s.q.head_stride) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(q), y = *reinterpret_cast<const uint32_t*>(q + 2);
-            const float2 f = floats<T>(x), e = floats<T>(y);
-            const float v[4] = {f.x, f.y, e.x, e.y};
+            for (int h = 0; h < G; ++h, q += s.q.head_stride) {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(q), y = *reinterpret_cast<const uint32_t*>(q + 2);
+              const float2 f = floats<T>(x), e = floats<T>(y);
+              const float v[4] = {f.x, f.y, e.x, e.y};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const double w = v[i];
-              if (v[i] < 0.f)
-                down[i] += w;
-              else
-                up[i] += w;
+              for (int i = 0; i < 4; ++i) {
+                const double w = v[i];
+                if (v[i] < 0.f)
+                  down[i] += w;
+                else
+                  up[i] += w;
+              }
             }
           }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            above_on[p][i] = (up[2 * i] != 0 ? 0xffffu : 0u) | (up[2 * i + 1] != 0 ? 0xffff0000u : 0u);
+            below_on[p][i] = (down[2 * i] != 0 ? 0xffffu : 0u) | (down[2 * i + 1] != 0 ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) above[p][i] = up[i] * Moved<T>::kHalf, below[p][i] = down[i] * Moved<T>::kHalf;
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          above_on[p][i] = (up[2 * i] != 0 ? 0xffffu : 0u) | (up[2 * i + 1] != 0 ? 0xffff0000u : 0u);
-          below_on[p][i] = (down[2 * i] != 0 ? 0xffffu : 0u) | (down[2 * i + 1] != 0 ? 0xffff0000u : 0u);
+      }
+      if (u + 1 < kUnits)
+        cp_wait<1>();
+      else
+        cp_wait<0>();
+      __syncwarp();
+      // this lane's channels of a row's bounds, those that count
+      const uint8_t* at = rows + (warp * kUnits + u) * kTogether * kRowBytes + lane * 8;
+      auto bounds_of = [&](int i, int p, uint2& top, uint2& low) {
+        top = low = make_uint2(0, 0);
+        if (p * kReach + lane * 4 < s.dim) {
+          const uint2 l = *reinterpret_cast<const uint2*>(at + i * kRowBytes + p * 256);
+          const uint2 h = *reinterpret_cast<const uint2*>(at + i * kRowBytes + p * 256 + s.dim * 2);
+          top = make_uint2(most2<T>(l.x, h.x) & above_on[p][0], most2<T>(l.y, h.y) & above_on[p][1]);
+          low = make_uint2(least2<T>(l.x, h.x) & below_on[p][0], least2<T>(l.y, h.y) & below_on[p][1]);
         }
+      };
+      double sum[kTogether];
+      uint32_t special = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) above[p][i] = up[i] * Moved<T>::kHalf, below[p][i] = down[i] * Moved<T>::kHalf;
+      for (int i = 0; i < kTogether; ++i) {
+        sum[i] = 0;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          uint2 top, low;
+          bounds_of(i, p, top, low);
+          special = zero_unless_special<T>(top.x, zero_unless_special<T>(top.y, special));
+          special = zero_unless_special<T>(low.x, zero_unless_special<T>(low.y, special));
+          sum[i] += above[p][0] * move<T>(top.x, 0);
+          sum[i] += above[p][1] * move<T>(top.x, 1);
+          sum[i] += above[p][2] * move<T>(top.y, 0);
+          sum[i] += above[p][3] * move<T>(top.y, 1);
+          sum[i] += below[p][0] * move<T>(low.x, 0);
+          sum[i] += below[p][1] * move<T>(low.x, 1);
+          sum[i] += below[p][2] * move<T>(low.y, 0);
+          sum[i] += below[p][3] * move<T>(low.y, 1);
+        }
       }
-    }
-    double sum[kTogether];
-    uint32_t special = 0;
-#pragma unroll
-    for (int i = 0; i < kTogether; ++i) {
-      sum[i] = 0;
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) {
-        const uint2 l = lo[i][p], u = hi[i][p];
-        hi[i][p] = make_uint2(most2<T>(l.x, u.x) & above_on[p][0], most2<T>(l.y, u.y) & above_on[p][1]);
-        lo[i][p] = make_uint2(least2<T>(l.x, u.x) & below_on[p][0], least2<T>(l.y, u.y) & below_on[p][1]);
-        special = zero_unless_special<T>(hi[i][p].x, zero_unless_special<T>(hi[i][p].y, special));
-        special = zero_unless_special<T>(lo[i][p].x, zero_unless_special<T>(lo[i][p].y, special));
-        sum[i] += above[p][0] * move<T>(hi[i][p].x, 0);
-        sum[i] += above[p][1] * move<T>(hi[i][p].x, 1);
-        sum[i] += above[p][2] * move<T>(hi[i][p].y, 0);
-        sum[i] += above[p][3] * move<T>(hi[i][p].y, 1);
-        sum[i] += below[p][0] * move<T>(lo[i][p].x, 0);
-        sum[i] += below[p][1] * move<T>(lo[i][p].x, 1);
-        sum[i] += below[p][2] * move<T>(lo[i][p].y, 0);
-        sum[i] += below[p][3] * move<T>(lo[i][p].y, 1);
-      }
-    }
-    double by = Moved<T>::kHalf;
-    if (__any_sync(0xffffffffu, special & 0x7fff7fffu)) {
-      by = 1 / Moved<T>::kHalf;
-#pragma unroll 1
-      for (int p = 0; p < PARTS; ++p)
+      // (rows of blocks that are not there hold what was there before: nobody reads their scores)
+      double by = Moved<T>::kHalf;
+      if (__any_sync(0xffffffffu, special & 0x7fff7fffu)) {
+        by = 1 / Moved<T>::kHalf;
 #pragma unroll
         for (int i = 0; i < kTogether; ++i) {
-          const uint2 u = PARTS > 1 && p ? hi[i][PARTS - 1] : hi[i][0], l = PARTS > 1 && p ? lo[i][PARTS - 1] : lo[i][0];
-          const float2 v[4] = {floats<T>(u.x), floats<T>(u.y), floats<T>(l.x), floats<T>(l.y)};
-          if (p == 0) sum[i] = 0;
+          sum[i] = 0;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const double a0 = PARTS > 1 && p ? above[PARTS - 1][2 * x] : above[0][2 * x],
-                         a1 = PARTS > 1 && p ? above[PARTS - 1][2 * x + 1] : above[0][2 * x + 1],
-                         b0 = PARTS > 1 && p ? below[PARTS - 1][2 * x] : below[0][2 * x],
-                         b1 = PARTS > 1 && p ? below[PARTS - 1][2 * x + 1] : below[0][2 * x + 1];
-            sum[i] += a0 * v[x].x + a1 * v[x].y + (b0 * v[2 + x].x + b1 * v[2 + x].y);
+          for (int p = 0; p < PARTS; ++p) {
+            uint2 top, low;
+            bounds_of(i, p, top, low);
+            const float2 a0 = floats<T>(top.x), a1 = floats<T>(top.y), b0 = floats<T>(low.x), b1 = floats<T>(low.y);
+            sum[i] += above[p][0] * a0.x + above[p][1] * a0.y + above[p][2] * a1.x + above[p][3] * a1.y;
+            sum[i] += below[p][0] * b0.x + below[p][1] * b0.y + below[p][2] * b1.x + below[p][3] * b1.y;
           }
         }
-    }
-    // halve the eight sums while the lanes are added: lane bits 4, 3 and 2 choose the block
-#pragma unroll
-    for (int width = kTogether / 2, bit = 16; width > 0; width /= 2, bit /= 2)
-#pragma unroll
-      for (int i = 0; i < width; ++i) {
-        const bool upper = lane & bit;
-        const double give = upper ? sum[i] : sum[i + width], keep = upper ? sum[i + width] : sum[i];
-        sum[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
       }
-    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 2);
-    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
-    const int j = j0 + (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
-    if ((lane & 3) == 0 && j < n)
-      s.scores[(static_cast<long long>(b) * s.kv_heads + g) * s.req.width + j] = static_cast<float>(sum[0] * by);
+      // halve the eight sums while the lanes are added: lane bits 4, 3 and 2 choose the block
+#pragma unroll
+      for (int width = kTogether / 2, bit = 16; width > 0; width /= 2, bit /= 2)
+#pragma unroll
+        for (int i = 0; i < width; ++i) {
+          const bool upper = lane & bit;
+          const double give = upper ? sum[i] : sum[i + width], keep = upper ? sum[i + width] : sum[i];
+          sum[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+        }
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 2);
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+      const int j = j0 + (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
+      if ((lane & 3) == 0 && j < n)
+        s.scores[(static_cast<long long>(b) * s.kv_heads + g) * s.req.width + j] = static_cast<float>(sum[0] * by);
+    }
+    __syncwarp();  // the rows have been read
   }
 }
 
@@ -589,25 +621,31 @@ cudaError_t paged_kv_bounds(const PagedKv& kv, const KvRequests& req, int new_to
 cudaError_t paged_kv_select(const KvSelect& s, cudaStream_t stream) {
   if (s.req.requests == 0) return cudaSuccess;
   if (s.req.width) {
-    const dim3 grid((s.req.width + kScoreBlocks - 1) / kScoreBlocks, s.req.requests);
+    const int64_t units = (s.req.width + kTogether - 1ll) / kTogether * s.kv_heads;
+    const int64_t items = (units / kScoreWarps + 1) * s.req.requests;
+    if (units > INT_MAX || items > INT_MAX || s.req.requests > kMostRequests) return cudaErrorInvalidValue;
+    constexpr int kBytes = kScoreWarps * 2 * kTogether * kReach * 4;  // two units, or one of twice the length
     auto score = s.type == kKvBf16 ? (s.dim <= kReach ? score_kernel<__nv_bfloat16, 1> : score_kernel<__nv_bfloat16, 2>)
                                    : (s.dim <= kReach ? score_kernel<__half, 1> : score_kernel<__half, 2>);
-    score<<<grid, kScoreWarps * 32, 0, stream>>>(s);
-    const cudaError_t rc = cudaGetLastError();
+    static std::atomic<uint64_t> ready[4];  // devices that know the kernels' shared memory
+    const int which = (s.type == kKvBf16) + 2 * (s.dim <= kReach);
+    int device = 0, sms = 0;
+    cudaError_t rc = sm_count(&sms, &device);
+    if (rc != cudaSuccess) return rc;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(ready[which].load(std::memory_order_relaxed) & bit)) {
+      rc = cudaFuncSetAttribute(score, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes + (kMostRequests + 1) * 4);
+      if (rc != cudaSuccess) return rc;
+      ready[which].fetch_or(bit, std::memory_order_relaxed);
+    }
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, 3 * sms));  // three CTAs to an SM
+    score<<<grid, kScoreWarps * 32, kBytes + (s.req.requests + 1) * 4, stream>>>(s, FastDiv::make(s.block), FastDiv::make(s.kv_heads));
+    rc = cudaGetLastError();
     if (rc != cudaSuccess) return rc;
   }
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(s.req.requests * s.kv_heads);
-  config.stream = stream;
-  cudaLaunchAttribute attr;  // it waits for the scores itself
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = s.req.width ? 1 : 0;
   cudaError_t rc = cudaSuccess;
   for_width(s.req.width, [&](auto threads, auto items) {
-    config.blockDim = dim3(threads());
-    rc = cudaLaunchKernelEx(&config, select_kernel<threads(), items()>, s);
+    rc = launch_after(select_kernel<threads(), items()>, s.req.requests * s.kv_heads, threads(), stream, s);
   });
   return rc;
 }

@@ -10,6 +10,8 @@
 
 namespace ppb {
 
+constexpr int kMostRequests = 4096;
+
 enum KvType : int { kKvBf16 = 0, kKvFp16 = 1 };
 
 // One layer's cache [2, pages, block, kv_heads, dim]: K, and V `lane_stride`
@@ -22,7 +24,7 @@ struct PagedKv {
   int type = kKvBf16;
 };
 
-// At most 4096 requests: their block table (int32, `width` entries a row) and lengths.
+// At most kMostRequests requests: their block table (int32, `width` entries a row) and lengths.
 // An entry outside [0, pages) is a block that is not resident: its tokens are
 // left out.  Lengths are cut to the table's width * block.
 struct KvRequests {
