@@ -53,30 +53,59 @@ __device__ __forceinline__ float2 floats(uint32_t v) {
 }
 
 // ---- key bounds -------------------------------------------------------------------
-// A CTA for each block: a thread takes 8 channels of all its tokens, 16 bytes a load,
-// eight loads in flight; the keys' bytes bound it.
+// A CTA for each block in turn, of those that there are: a thread takes 8 channels of
+// 16 tokens at a time, 16 loads of 16 bytes in flight, and the next block's page is
+// looked up meanwhile.  The keys' bytes bound it.
+constexpr int kBoundsRows = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ PagedKv kv, const __grid_constant__ KvRequests r,
-                                                     int new_tokens, T* __restrict__ bounds) {
-  const int b = blockIdx.y, len = length_of(r, kv.block, b);
-  const int j = (new_tokens < 0 ? 0 : max(0, len - new_tokens) / kv.block) + blockIdx.x;
-  if (static_cast<long long>(j) * kv.block >= len) return;
-  const int page = r.table[b * r.table_stride + j], n = min(kv.block, len - j * kv.block);
-  if (page < 0 || page >= kv.pages) return;
+__global__ void __launch_bounds__(256, 2)
+    bounds_kernel(const __grid_constant__ PagedKv kv, const __grid_constant__ KvRequests r, FastDiv by_block, int new_tokens,
+                  T* __restrict__ bounds) {
+  extern __shared__ uint32_t starts[];  // of the requests' blocks that are due
+  __shared__ uint32_t scratch[8];
+  auto from = [&](int len) { return new_tokens < 0 ? 0 : static_cast<int>(by_block.quotient(max(0, len - new_tokens))); };
+  running_sums(r.requests,
+               [&](int b) {
+                 const int len = length_of(r, kv.block, b);
+                 return by_block.quotient(len + kv.block - 1) - (len > 0 ? from(len) : 0);
+               },
+               starts, scratch);
+  struct Due {
+    int page, tokens;
+  };
+  auto look_up = [&](uint32_t item) {
+    if (item >= starts[r.requests]) return Due{-1, 0};
+    const int b = request_of(starts, r.requests, item), len = length_of(r, kv.block, b);
+    const int j = from(len) + static_cast<int>(item - starts[b]);
+    return Due{r.table[b * r.table_stride + j], min(kv.block, len - j * kv.block)};
+  };
   const int per = kv.dim / 8;
-  for (int c = threadIdx.x; c < kv.kv_heads * per; c += blockDim.x) {
-    const int g = c / per, d = c % per * 8;
-    const T* k = static_cast<const T*>(kv.base) + page * kv.page_stride + g * kv.head_stride + d;
-    uint4 lo = __ldcs(reinterpret_cast<const uint4*>(k)), hi = lo;
-#pragma unroll 8
-    for (int t = 1; t < n; ++t) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(k + t * kv.token_stride));
-      lo = make_uint4(least2<T>(lo.x, v.x), least2<T>(lo.y, v.y), least2<T>(lo.z, v.z), least2<T>(lo.w, v.w));
-      hi = make_uint4(most2<T>(hi.x, v.x), most2<T>(hi.y, v.y), most2<T>(hi.z, v.z), most2<T>(hi.w, v.w));
+  Due next = look_up(blockIdx.x);
+  for (uint32_t item = blockIdx.x; item < starts[r.requests]; item += gridDim.x) {
+    const Due due = next;
+    next = look_up(item + gridDim.x);
+    if (due.page < 0 || due.page >= kv.pages) continue;
+    for (int c = threadIdx.x; c < kv.kv_heads * per; c += blockDim.x) {
+      const int g = c / per, d = (c - g * per) * 8;
+      const T* k = static_cast<const T*>(kv.base) + due.page * kv.page_stride + g * kv.head_stride + d;
+      uint4 lo, hi;
+      for (int t0 = 0; t0 < due.tokens; t0 += kBoundsRows) {
+        uint4 v[kBoundsRows];
+#pragma unroll
+        for (int i = 0; i < kBoundsRows; ++i)  // behind the last token its row again
+          v[i] = __ldcs(reinterpret_cast<const uint4*>(k + min(t0 + i, due.tokens - 1) * kv.token_stride));
+        if (t0 == 0) lo = hi = v[0];
+#pragma unroll
+        for (int i = 0; i < kBoundsRows; ++i) {
+          lo = make_uint4(least2<T>(lo.x, v[i].x), least2<T>(lo.y, v[i].y), least2<T>(lo.z, v[i].z), least2<T>(lo.w, v[i].w));
+          hi = make_uint4(most2<T>(hi.x, v[i].x), most2<T>(hi.y, v[i].y), most2<T>(hi.z, v[i].z), most2<T>(hi.w, v[i].w));
+        }
+      }
+      T* o = bounds + (static_cast<long long>(due.page) * kv.kv_heads + g) * 2 * kv.dim + d;
+      *reinterpret_cast<uint4*>(o) = lo;
+      *reinterpret_cast<uint4*>(o + kv.dim) = hi;
     }
-    T* o = bounds + (static_cast<long long>(page) * kv.kv_heads + g) * 2 * kv.dim + d;
-    *reinterpret_cast<uint4*>(o) = lo;
-    *reinterpret_cast<uint4*>(o + kv.dim) = hi;
   }
 }
 
@@ -606,15 +635,20 @@ void for_width(int width, Launch launch) {
 
 cudaError_t paged_kv_bounds(const PagedKv& kv, const KvRequests& req, int new_tokens, void* bounds,
                             cudaStream_t stream) {
-  const int blocks = new_tokens < 0 ? req.width
-                                    : static_cast<int>(std::min((long long)req.width, (new_tokens + kv.block - 2ll) / kv.block + 1));
+  const int64_t blocks = new_tokens < 0 ? req.width : std::min<int64_t>(req.width, (new_tokens + kv.block - 2ll) / kv.block + 1);
   if (req.requests == 0 || blocks == 0 || new_tokens == 0) return cudaSuccess;
-  const dim3 grid(blocks, req.requests);
-  const int threads = std::min(256, (kv.kv_heads * kv.dim / 8 + 31) / 32 * 32);
+  if (req.requests > kMostRequests) return cudaErrorInvalidValue;
+  int sms = 0, device = 0;
+  const cudaError_t rc = sm_count(&sms, &device);
+  if (rc != cudaSuccess) return rc;
+  const int threads = std::min<int64_t>(256, (static_cast<int64_t>(kv.kv_heads) * kv.dim / 8 + 31) / 32 * 32);
+  const int64_t ctas = std::min<int64_t>(blocks * req.requests, sms * (512 / threads));
+  const int smem = (req.requests + 1) * 4;
+  const FastDiv by_block = FastDiv::make(kv.block);
   if (kv.type == kKvBf16)
-    bounds_kernel<<<grid, threads, 0, stream>>>(kv, req, new_tokens, static_cast<__nv_bfloat16*>(bounds));
+    bounds_kernel<<<ctas, threads, smem, stream>>>(kv, req, by_block, new_tokens, static_cast<__nv_bfloat16*>(bounds));
   else
-    bounds_kernel<<<grid, threads, 0, stream>>>(kv, req, new_tokens, static_cast<__half*>(bounds));
+    bounds_kernel<<<ctas, threads, smem, stream>>>(kv, req, by_block, new_tokens, static_cast<__half*>(bounds));
   return cudaGetLastError();
 }
 
