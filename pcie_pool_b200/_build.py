@@ -1,4 +1,5 @@
-"""In-tree build of the native core ``pcie_pool_b200._C``.
+"""In-tree build of the native modules ``pcie_pool_b200._C`` (the core) and
+``pcie_pool_b200._kv`` (the paged-KV operators' entry points on torch tensors).
 
 CUDA sources are compiled by nvcc for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``); host sources by g++.  The CUDA
@@ -26,15 +27,25 @@ CSRC = PKG_DIR / "csrc"
 BUILD_DIR = PKG_DIR / "_build"
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 
-CU_SOURCES = ["ppb_common.cu", "pool_kernels.cu", "engine.cu", "native_ops.cu", "noalloc.cu", "vmm.cu",
-              "kv_attention.cu", "kv_blocks.cu"]
-CC_SOURCES = ["planner.cc", "host_ops.cc", "bindings.cc", "bind_ops.cc", "bind_kv.cc"]
+CU_SOURCES = ["ppb_common.cu", "pool_kernels.cu", "engine.cu", "native_ops.cu", "noalloc.cu", "vmm.cu"]
+CC_SOURCES = ["planner.cc", "host_ops.cc", "bindings.cc", "bind_ops.cc"]
+# the paged-KV operators: a module of its own, since it is built against torch's library
+KV_CU_SOURCES = ["kv_attention.cu", "kv_blocks.cu"]
+KV_CC_SOURCES = ["torch_kv.cc"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
-def extension_path() -> Path:
+def extension_path(name: str = "_C") -> Path:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    return PKG_DIR / f"_C{suffix}"
+    return PKG_DIR / f"{name}{suffix}"
+
+
+def _torch_paths() -> tuple[str, Path]:
+    """torch's version and folder, without importing it."""
+    import importlib.metadata
+    import importlib.util
+
+    return importlib.metadata.version("torch"), Path(importlib.util.find_spec("torch").submodule_search_locations[0])
 
 
 def _includes() -> list[str]:
@@ -69,41 +80,48 @@ def _compile(cmd: list[str]) -> None:
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile (if needed) and link ``_C``; returns the extension path."""
+    """Compile (if needed) and link ``_C`` and ``_kv``; returns ``_C``'s path."""
     BUILD_DIR.mkdir(exist_ok=True)
     nvcc = str(CUDA_HOME / "bin" / "nvcc")
     inc = _includes()
     head = _newest_header()
+    version, torch_dir = _torch_paths()
+    torch_inc = [f"-I{CSRC}", f"-isystem{torch_dir / 'include'}", f"-isystem{torch_dir / 'include/torch/csrc/api/include'}",
+                 f"-I{sysconfig.get_paths()['include']}", f"-I{CUDA_HOME / 'include'}"]
     cmds: list[list[str]] = []
-    objs: list[Path] = []
-    for name in CU_SOURCES:
-        src = CSRC / name
-        obj = BUILD_DIR / (name + ".o")
-        objs.append(obj)
-        if force or _stale(src, obj, head):
-            cmds.append(
-                [nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-                 "-Xcompiler", "-fvisibility=hidden", *inc, "-c", str(src), "-o", str(obj)]
-            )
-    for name in CC_SOURCES:
-        src = CSRC / name
-        obj = BUILD_DIR / (name + ".o")
-        objs.append(obj)
-        if force or _stale(src, obj, head):
-            cmds.append(
-                ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", *inc, "-c", str(src),
-                 "-o", str(obj)]
-            )
+
+    def objects(names: list[str], compiler: list[str], includes: list[str], tag: str = "") -> list[Path]:
+        objs = []
+        for name in names:
+            src, obj = CSRC / name, BUILD_DIR / f"{name}{tag}.o"
+            objs.append(obj)
+            if force or _stale(src, obj, head):
+                cmds.append([*compiler, *includes, "-c", str(src), "-o", str(obj)])
+        return objs
+
+    cuda = [nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
+    host = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden"]
+    core = objects(CU_SOURCES, cuda, inc) + objects(CC_SOURCES, host, inc)
+    core_changed = bool(cmds)
+    kv = objects(KV_CU_SOURCES, cuda, [f"-I{CSRC}"])
+    # its objects are one torch version's
+    kv += objects(KV_CC_SOURCES, [*host, "-DTORCH_EXTENSION_NAME=_kv"], torch_inc, f".torch-{version}")
+    kv_changed = any(str(o) in c for c in cmds for o in kv)
     if cmds:
         with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 4)) as pool:
             list(pool.map(_compile, cmds))
+    cudart = [f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static", "-lrt", "-lpthread", "-ldl"]
     out = extension_path()
-    if force or cmds or not out.exists():
-        link = ["g++", "-shared", "-o", str(out), *map(str, objs),
-                f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static", "-lrt", "-lpthread", "-ldl"]
-        _compile(link)
+    if force or core_changed or not out.exists():
+        _compile(["g++", "-shared", "-o", str(out), *map(str, core), *cudart])
+    kv_out, stamp = extension_path("_kv"), BUILD_DIR / "_kv.torch"
+    if force or kv_changed or not kv_out.exists() or not stamp.exists() or stamp.read_text() != version:
+        # torch is imported before the module: its libraries are found by their names
+        _compile(["g++", "-shared", "-o", str(kv_out), *map(str, kv), f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda",
+                  "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,--exclude-libs,ALL", *cudart])
+        stamp.write_text(version)
     if verbose:
-        print(f"built {out}")
+        print(f"built {out} and {kv_out}")
     return out
 
 

@@ -1,4 +1,4 @@
-"""Loader for the native core ``pcie_pool_b200._C``.
+"""Loader for the native modules ``pcie_pool_b200._C`` and ``pcie_pool_b200._kv``.
 
 On a machine with a visible GPU a missing or broken extension is an error
 (raised on first use), never a silent fallback to a slower path.
@@ -11,6 +11,7 @@ import os
 from types import ModuleType
 
 _MOD: ModuleType | None = None
+_KV: ModuleType | None = None
 _ERR: BaseException | None = None
 
 
@@ -22,20 +23,34 @@ def _gpu_visible() -> bool:
 
 def native(build_if_missing: bool = True) -> ModuleType:
     """Return the loaded extension module, building it in-tree if needed."""
-    global _MOD, _ERR
-    if _MOD is not None:
-        return _MOD
+    global _MOD
+    if _MOD is None:
+        _MOD = _load("pcie_pool_b200._C", build_if_missing)
+    return _MOD
+
+
+def native_kv() -> ModuleType:
+    """Return ``pcie_pool_b200._kv``, the paged-KV operators on torch tensors,
+    building it in-tree if needed."""
+    global _KV
+    if _KV is None:
+        import torch  # noqa: F401  (its libraries are the module's)
+
+        _KV = _load("pcie_pool_b200._kv", True)
+    return _KV
+
+
+def _load(name: str, build_if_missing: bool) -> ModuleType:
+    global _ERR
     try:
-        _MOD = importlib.import_module("pcie_pool_b200._C")
-        return _MOD
+        return importlib.import_module(name)
     except ImportError as exc:  # pragma: no cover - depends on build state
         _ERR = exc
     if build_if_missing and os.environ.get("PCIE_POOL_NO_BUILD") != "1":
         from . import _build
 
         _build.build()
-        _MOD = importlib.import_module("pcie_pool_b200._C")
-        return _MOD
+        return importlib.import_module(name)
     raise RuntimeError(
         "pcie_pool_b200 native extension is not built; run "
         "`python -m pcie_pool_b200._build`"

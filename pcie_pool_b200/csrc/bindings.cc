@@ -33,7 +33,6 @@ std::vector<T> to_vec(const py::array_t<T, py::array::c_style | py::array::force
 
 void bind_ops(py::module_& m);
 void bind_planner(py::module_& m);
-void bind_kv(py::module_& m);
 
 PYBIND11_MODULE(_C, m) {
   m.doc() = "pcie_pool_b200 native core (sm_100a kernels + PoolEngine)";
@@ -283,5 +282,4 @@ PYBIND11_MODULE(_C, m) {
 
   bind_ops(m);
   bind_planner(m);
-  bind_kv(m);
 }

@@ -626,37 +626,35 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4)
 
 int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
-
-// The workspace's parts behind `base`; returns its size.
-uint64_t lay_out(int requests, int width, int block, int heads, int kv_heads, int dim, bool mass, int sms, void* base,
-                 Work& w) {
-  const int G = heads / kv_heads, warps = sms * (padded(dim) == 256 ? Shape<256>::kWarps : Shape<128>::kWarps);
+// The workspace's parts behind a.work; returns its size.
+uint64_t lay_out(const KvAttention& a, int sms, Work& w) {
+  const int dim = a.kv.dim, heads = a.q.heads, requests = a.req.requests, G = heads / a.kv.kv_heads;
+  const int warps = sms * (padded(dim) == 256 ? Shape<256>::kWarps : Shape<128>::kWarps);
   w.shared = G;
   w.groups_each = (G + kRowGroup - 1) / kRowGroup;
-  w.groups = kv_heads * w.groups_each;
+  w.groups = a.kv.kv_heads * w.groups_each;
   w.rows = G <= 8 ? 8 : 16;
   w.most_ranges = warps / w.groups > 0 ? warps / w.groups : 1;
   w.by_ranges = FastDiv::make(w.most_ranges);
-  w.by_block = FastDiv::make(block);
+  w.by_block = FastDiv::make(a.kv.block);
   w.by_groups = FastDiv::make(w.groups);
   w.by_groups_each = FastDiv::make(w.groups_each);
-  w.max_tiles = static_cast<int>((static_cast<int64_t>(width) * block + kTile - 1) / kTile);
-  w.mass_ctas = mass ? (width + kMassBlocks - 1) / kMassBlocks : 0;
-  const uint64_t parts = 2ull * w.most_ranges * w.groups * w.rows;
-  uint8_t* p = static_cast<uint8_t*>(base);
-  uint64_t at = 0;
-  w.part_o = reinterpret_cast<float*>(p + at);
-  at += up(parts * dim * 4);
-  w.part_ml = reinterpret_cast<float2*>(p + at);
-  at += up(parts * 8);
-  w.first = reinterpret_cast<uint32_t*>(p + at);
-  at += up((requests + 1ull) * 4);
+  w.max_tiles = static_cast<int>((static_cast<int64_t>(a.req.width) * a.kv.block + kTile - 1) / kTile);
+  w.mass_ctas = a.mass ? (a.req.width + kMassBlocks - 1) / kMassBlocks : 0;
   w.by_cut = requests >= w.most_ranges;
-  w.items = reinterpret_cast<int4*>(p + at);
-  at += up((w.by_cut ? w.most_ranges : requests) * 16ull);
-  w.z = mass ? reinterpret_cast<float*>(p + at) : nullptr;
-  if (mass) at += up(uint64_t(requests) * w.max_tiles * heads * 4);
+  const uint64_t parts = 2ull * w.most_ranges * w.groups * w.rows;
+  uint8_t* p = static_cast<uint8_t*>(a.work);
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    uint8_t* here = p + at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  w.part_o = reinterpret_cast<float*>(take(parts * dim * 4));
+  w.part_ml = reinterpret_cast<float2*>(take(parts * 8));
+  w.first = reinterpret_cast<uint32_t*>(take((requests + 1ull) * 4));
+  w.items = reinterpret_cast<int4*>(take((w.by_cut ? w.most_ranges : requests) * 16ull));
+  w.z = a.mass ? reinterpret_cast<float*>(take(uint64_t(requests) * w.max_tiles * heads * 4)) : nullptr;
   return at;
 }
 
@@ -713,11 +711,10 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
 
 }  // namespace
 
-uint64_t paged_kv_attention_work(int requests, int width, int block, int heads, int kv_heads, int dim, bool mass) {
+uint64_t paged_kv_attention_work(const KvAttention& a) {
   int sms = 0, device = 0;
   Work w;
-  if (sm_count(&sms, &device) != cudaSuccess) return 0;
-  return lay_out(requests, width, block, heads, kv_heads, dim, mass, sms, nullptr, w);
+  return sm_count(&sms, &device) == cudaSuccess ? lay_out(a, sms, w) : 0;
 }
 
 cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream) {
@@ -727,7 +724,7 @@ cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream) {
   cudaError_t rc = sm_count(&sms, &device);
   if (rc != cudaSuccess) return rc;
   Work w;
-  lay_out(a.req.requests, a.req.width, a.kv.block, a.q.heads, a.kv.kv_heads, a.kv.dim, a.mass != nullptr, sms, a.work, w);
+  lay_out(a, sms, w);
   rc = a.kv.type == kKvBf16 ? launch<__nv_bfloat16>(a, w, sms, device, stream)
                              : launch<__half>(a, w, sms, device, stream);
   return rc;

@@ -56,8 +56,8 @@ struct KvAttention {
   void* work = nullptr;    // paged_kv_attention_work() bytes
 };
 
-// Workspace bytes of a call on the current device.
-uint64_t paged_kv_attention_work(int requests, int width, int block, int heads, int kv_heads, int dim, bool mass);
+// Workspace bytes of a call on the current device (nothing that `a` points to is read).
+uint64_t paged_kv_attention_work(const KvAttention& a);
 cudaError_t paged_kv_attention(const KvAttention& a, cudaStream_t stream);
 
 // Bounds [pages, kv_heads, 2, dim] (smallest, then largest key of each channel) of

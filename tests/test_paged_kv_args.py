@@ -130,14 +130,13 @@ def test_evict_refuses(good):
 
 
 def test_a_query_that_splits_pairs_is_copied(good):
-    from pcie_pool_b200.ops.paged_kv import _query
+    from pcie_pool_b200._native import native_kv
 
     q = good["q"]
     odd = torch.zeros(q.numel() + 1, dtype=q.dtype)[1:].view(q.shape).copy_(q)
     spread = torch.zeros(*q.shape, 2, dtype=q.dtype)[..., 0].copy_(q)
     rows = torch.zeros(2, 8, 65, dtype=q.dtype)[..., :64].copy_(q)
     for x in (odd, spread, rows):
-        got, (at, row, head, heads) = _query(torch, x, -1, q.dtype, 64, 2, 2)
-        assert (at, row, head, heads) == (got.data_ptr(), 512, 64, 8)
+        got = native_kv().whole_pairs(x)
         assert got.data_ptr() % 4 == 0 and got.is_contiguous() and torch.equal(got, q)
-    assert _query(torch, q, -1, q.dtype, 64, 2, 2)[0] is q
+    assert native_kv().whole_pairs(q).data_ptr() == q.data_ptr()
