@@ -118,7 +118,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     if force or kv_changed or not kv_out.exists() or not stamp.exists() or stamp.read_text() != version:
         # torch is imported before the module: its libraries are found by their names
         _compile(["g++", "-shared", "-o", str(kv_out), *map(str, kv), f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda",
-                  "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,--exclude-libs,ALL", *cudart])
+                  "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,--exclude-libs,ALL", *cudart])
         stamp.write_text(version)
     if verbose:
         print(f"built {out} and {kv_out}")

@@ -4,6 +4,7 @@
 // 10 us on the device: with checks and allocations in Python it took 17 us of the host's
 // time, half of it for those.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -51,6 +52,11 @@ cudaStream_t stream_of(std::initializer_list<const Tensor*> tensors) {
       need(!x->requires_grad(), "the paged-KV operators have no gradient: call them under torch.no_grad()");
   need(t.is_cuda(), "the tensors must be on a CUDA device");
   return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+}
+
+// at::empty without its way through the dispatcher, which is half of its time.
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+  return at::detail::empty_cuda(sizes, type, device, std::nullopt);
 }
 
 KvRequests requests_of(const Tensor& table, const Tensor& lens, const at::Device& device, int64_t block) {
@@ -143,15 +149,15 @@ py::object kv_attention(const Tensor& given, const Tensor& kv, const Tensor& tab
     need(!overlaps(*out, q) && !overlaps(*out, kv), "out must not overlap q or kv");
   }
   const cudaStream_t stream = stream_of({&kv, &q});
-  if (!out) out = at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous);
-  const Tensor lse = at::empty({n, a.q.heads}, q.options().dtype(at::kFloat));
+  if (!out) out = empty(q.sizes(), q.scalar_type(), device);
+  const Tensor lse = empty({n, a.q.heads}, at::kFloat, device);
   if (blocks && a.blocks_width == 0) {
     out->zero_();
     lse.fill_(-INFINITY);
   } else {
     DeviceGuard guard(device.index());
     const int64_t bytes = paged_kv_attention_work(a);
-    const Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
+    const Tensor work = empty({bytes}, at::kByte, device);
     a.out = out->data_ptr();
     a.lse = lse.data_ptr<float>();
     a.work = work.data_ptr();
@@ -195,8 +201,8 @@ Tensor kv_select(const Tensor& given, const Tensor& bounds, const Tensor& table,
   s.recent = whole(recent, 0, "recent must be an integer >= 0");
   need(int64_t(s.sink) + s.recent <= s.keep, "keep must be at least sink + recent");
   const cudaStream_t stream = stream_of({&bounds, &q});
-  const Tensor out = at::empty({s.req.requests, s.kv_heads, s.keep}, table.options());
-  const Tensor scores = at::empty({int64_t(s.req.requests) * s.kv_heads * s.req.width}, q.options().dtype(at::kFloat));
+  const Tensor out = empty({s.req.requests, s.kv_heads, s.keep}, at::kInt, bounds.device());
+  const Tensor scores = empty({int64_t(s.req.requests) * s.kv_heads * s.req.width}, at::kFloat, bounds.device());
   s.out = out.data_ptr<int>();
   s.scores = scores.data_ptr<float>();
   DeviceGuard guard(bounds.get_device());
@@ -221,9 +227,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> kv_evict(const Tensor
   need(int64_t(e.sink) + e.recent <= e.budget, "budget must be at least sink + recent");
   const cudaStream_t stream = stream_of({&mass});
   const at::IntArrayRef rows = table.sizes();
-  Tensor kept = at::empty(rows, table.options()), gone = at::empty(rows, table.options()), places = at::empty(rows, table.options());
-  Tensor new_mass = at::empty(rows, mass.options());
-  Tensor new_lens = at::empty(lens.sizes(), lens.options()), count = at::empty(lens.sizes(), lens.options());
+  const at::Device device = mass.device();
+  const Tensor kept = empty(rows, at::kInt, device), gone = empty(rows, at::kInt, device), places = empty(rows, at::kInt, device);
+  const Tensor new_mass = empty(rows, at::kFloat, device);
+  const Tensor new_lens = empty(lens.sizes(), at::kInt, device), count = empty(lens.sizes(), at::kInt, device);
   e.new_table = kept.data_ptr<int>();
   e.new_lens = new_lens.data_ptr<int>();
   e.new_mass = new_mass.data_ptr<float>();
