@@ -7,7 +7,7 @@ from ..offload_store import AdapterTransferContext, ReceiptTransferHandle
 from .base import FrameworkAdapter
 from .inference import (FrameworkKVSlot, FrameworkKVSlotAdapter, InferenceKVSlot, InferenceKVSlotAdapter,
                         make_contiguous_kv_slots)
-from .kv_offload import KVTransferStats, PagedKVOffloader
+from .kv_offload import EvictedKV, KVTransferStats, PagedKVOffloader
 from .model_loading import ModelLoader, ModelWeightLoader
 from .streamed_optimizer import StepStats, StreamedAdamW
 from .training_offload import TrainingOffloadManager, TrainingOffloadStore
@@ -21,7 +21,7 @@ from .vllm_kv_connector import (TurboBusConnector, TurboBusConnectorConfig, Turb
                                 clear_saved_prefixes, get_connector_events, get_saved_prefix)
 
 __all__ = [
-    "AdapterTransferContext", "FrameworkAdapter", "FrameworkKVSlot", "FrameworkKVSlotAdapter", "InferenceKVSlot",
+    "AdapterTransferContext", "EvictedKV", "FrameworkAdapter", "FrameworkKVSlot", "FrameworkKVSlotAdapter", "InferenceKVSlot",
     "InferenceKVSlotAdapter", "KVTransferStats", "ModelLoader", "ModelWeightLoader", "PagedKVOffloader",
     "ReceiptTransferHandle", "TrainingOffloadManager", "TrainingOffloadStore", "TurboBusConnector",
     "TurboBusConnectorConfig", "TurboBusConnectorMetadata", "TurboBusRequestMetadata", "TurboBusSavedPrefix",

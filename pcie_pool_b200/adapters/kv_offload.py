@@ -43,7 +43,45 @@ def kv_segments(nunits: int, host_off: int, span_blocks: int | None, nblocks: in
     return [(host_off + s * span_blocks * unit_bytes, s * nblocks, nblocks) for s in range(spans)]
 
 
-class PagedKVOffloader:
+@dataclass
+class EvictedKV:
+    """Blocks that left a request for the host: their pages and places in the
+    request's old table, where they were saved, and the transfer."""
+
+    request: int
+    blocks: list
+    index: list
+    host_off: int
+    stats: KVTransferStats
+
+
+class _EvictsKV:
+    """Eviction by accumulated attention weight, for what has ``save`` and ``prefix_bytes``."""
+
+    def evict(self, mass, block_table, context_lens, budget: int, *host, block_size: int, host_off: int = 0,
+              sink: int = 1, recent: int = 1):
+        """Cut every request to ``budget`` blocks (``ops.paged_kv_evict``: ``mass`` is what
+        ``ops.paged_kv_attention(mass=)`` added up) and save those that leave to the host, one
+        transfer for each request that loses any, one behind the other from ``host_off``; ``host``
+        is what ``save`` takes.  Returns (``KVEviction``, list of ``EvictedKV``): the requests go
+        on with the eviction's table, lengths and mass, the pages of ``EvictedKV.blocks`` are free,
+        and ``restore(pages, *host, host_off=...)`` brings a request's evicted blocks back."""
+        from ..ops import paged_kv_evict
+
+        e = paged_kv_evict(mass, block_table, context_lens, budget, block_size=block_size, sink=sink, recent=recent)
+        counts = e.evicted_count.tolist()
+        widest = max(counts, default=0)
+        pages, places = e.evicted_blocks[:, :widest].tolist(), e.evicted_index[:, :widest].tolist()
+        out = []
+        for b, n in enumerate(counts):
+            if n:
+                stats = self.save(pages[b][:n], *host, host_off=host_off)
+                out.append(EvictedKV(b, pages[b][:n], places[b][:n], host_off, stats))
+                host_off += self.prefix_bytes(n)
+        return e, out
+
+
+class PagedKVOffloader(_EvictsKV):
     """Save / restore vLLM-layout KV prefixes through a ``PoolEngine``."""
 
     def __init__(self, engine, kv_caches: Sequence, target: int, relays: Sequence[int] = (),
@@ -149,7 +187,7 @@ class PagedKVOffloader:
         return self._run(True, block_ids, host_ptr, host_bytes, host_off, span_blocks)
 
 
-class DaemonKVOffloader:
+class DaemonKVOffloader(_EvictsKV):
     """Save / restore vLLM-layout KV prefixes as daemon intents.
 
     Each save or restore is ONE intent whose landing spec asks the data plane
@@ -295,4 +333,4 @@ class DaemonKVOffloader:
         return self._run(True, block_ids, host, host_off, span_blocks)
 
 
-__all__ = ["DaemonKVOffloader", "KVTransferStats", "PagedKVOffloader", "kv_segments"]
+__all__ = ["DaemonKVOffloader", "EvictedKV", "KVTransferStats", "PagedKVOffloader", "kv_segments"]

@@ -67,7 +67,8 @@ KvRequests requests_of(const Tensor& table, const Tensor& lens, const at::Device
   need(table.device() == device && lens.device() == device, "all tensors must be on one CUDA device");
   need(block <= kMaxBlock, "at most 65536 tokens a block");
   need(width <= (kInt - 2 * kMaxBlock) / block, "block_table is too wide: a request has at most 2**31 tokens");
-  need(n * width * block < int64_t(1) << 34, "block_table is too large: at most 2**34 tokens in all");
+  need(n * width < kInt && n * width * block < int64_t(1) << 34,
+       "block_table is too large: at most 2**31 blocks and 2**34 tokens in all");
   need(width <= 1 || table.stride(1) == 1, "block_table's rows must be contiguous");
   need(n <= 1 || lens.stride(0) == 1, "context_lens must be contiguous");
   return {table.data_ptr<int>(), table.stride(0), lens.data_ptr<int>(), static_cast<int>(n), static_cast<int>(width)};

@@ -205,6 +205,32 @@ def test_sparse_attention_of_no_blocks(need_gpu):
         assert (out == 0).all() and (lse == -math.inf).all()
 
 
+@pytest.mark.parametrize("kv_heads,heads,dim", [(1300, 1300, 8), (300, 600, 256)])
+def test_more_key_heads_than_warps(need_gpu, kv_heads, heads, dim):
+    q, kv, table, lens = make(22, [40, 0, 17], 16, heads, kv_heads, dim, BF16)
+    mass = torch.zeros(table.shape, device="cuda") if heads <= 1024 else None
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), mass=mass, return_lse=True)
+    weight, lse_err = check_attention(q, kv, table, lens, out, lse)
+    if mass is not None:
+        tol = weight * (3 * lse_err.amax(1, keepdim=True) + (heads + 80) * 2.0 ** -24 + 2.0 ** -20)
+        assert ((mass.cpu().double() - weight).abs() <= tol + 2.0 ** -24 * weight).all()
+
+
+def test_nothing_to_do(need_gpu):
+    q, kv, table, lens = (t.cuda() for t in make(23, [40, 17], 16, 4, 2, 64, BF16))
+    bounds = torch.full((kv.shape[1], 2, 2, 64), 3.0, dtype=BF16, device="cuda")
+    none, mass = table[:, :0], torch.zeros(2, 0, device="cuda")
+    assert (ops.paged_kv_attention(q, kv, none, lens, mass=mass) == 0).all()
+    assert (ops.paged_kv_bounds(kv, none, lens, bounds) == 3).all()
+    assert (ops.paged_kv_select(q, bounds, none, lens, 4, block_size=16) == -1).all()
+    e = ops.paged_kv_evict(mass, none, lens, 4, block_size=16)
+    assert e.block_table.shape == (2, 0) and (e.context_lens == 0).all() and (e.evicted_count == 0).all()
+    empty = table[:0], lens[:0]
+    assert ops.paged_kv_select(q[:0], bounds, *empty, 4, block_size=16).shape == (0, 2, 4)
+    assert (ops.paged_kv_bounds(kv, *empty, bounds) == 3).all()
+    assert ops.paged_kv_evict(torch.zeros(0, table.shape[1], device="cuda"), *empty, 4, block_size=16).context_lens.shape == (0,)
+
+
 # ---- bounds ---------------------------------------------------------------------------------
 
 
@@ -392,6 +418,49 @@ def test_steps_with_a_bounded_cache_and_offload(need_gpu):
     assert ((joined - whole).abs() <= 2.0 ** -8 * (kept.abs() + back.abs() + whole.abs()) + 1e-4).all()
 
 
+def test_evicted_blocks_go_to_the_host_and_come_back(need_gpu):
+    """Two layers, cut by the mass that both add up; the blocks that leave are saved in the pooled data plane,
+    their pages overwritten, then restored into other pages: attention over all parts is as before."""
+    from pcie_pool_b200.adapters import PagedKVOffloader
+    from pcie_pool_b200.parallel.engine import PoolEngine
+    from pcie_pool_b200.utils.host_memory import PinnedHostBuffer
+
+    layers = [make(32 + i, [400, 37, 200], 16, 8, 2, 64, BF16, pages_extra=40) for i in range(2)]
+    table, lens = layers[0][2].cuda(), layers[0][3].cuda()
+    kvs = []
+    for q, kv, t, _ in layers:  # one table for all layers
+        g = torch.zeros_like(kv).cuda()
+        g[:, table.long()] = kv.cuda()[:, t.cuda().long()].nan_to_num(0.0)
+        kvs.append(g)
+    qs = [x[0].cuda() for x in layers]
+    mass = torch.zeros(table.shape, device="cuda")
+    whole = [ops.paged_kv_attention(q, kv, table, lens, mass=mass, return_lse=True) for q, kv in zip(qs, kvs)]
+    host = PinnedHostBuffer(1 << 20)
+    try:
+        store = PagedKVOffloader(PoolEngine([0], slot_bytes=1 << 20, slots=3, timeout_s=10.0), kvs, target=0)
+        e, gone = store.evict(mass, table, lens, 6, host.ptr, 1 << 20, block_size=16)
+        assert [(x.request, len(x.blocks)) for x in gone] == [(0, 19), (2, 7)]
+        free = [p for x in gone for p in x.blocks][::-1]
+        back = torch.full_like(table, -1)
+        for kv in kvs:
+            kv[:, free] = float("nan")  # the pages are used for something else
+        for x in gone:
+            pages, free = free[: len(x.blocks)], free[len(x.blocks):]
+            store.restore(pages, host.ptr, 1 << 20, host_off=x.host_off)
+            back[x.request, : len(pages)] = torch.tensor(pages, dtype=torch.int32)
+    finally:
+        host.release()
+    torch.cuda.synchronize()
+    for q, kv, (ref, ref_lse) in zip(qs, kvs, whole):
+        kept, kept_lse = ops.paged_kv_attention(q, kv, e.block_table, e.context_lens, return_lse=True)
+        rest, rest_lse = ops.paged_kv_attention(q, kv, back, e.evicted_count * 16, return_lse=True)
+        top = torch.logaddexp(kept_lse, rest_lse)
+        joined = (kept_lse - top).exp()[..., None] * kept + (rest_lse - top).exp()[..., None] * rest
+        assert torch.allclose(top, ref_lse, atol=1e-4)
+        # two roundings to bf16 of the parts and one of the whole
+        assert ((joined - ref).abs() <= 2.0 ** -8 * (kept.abs() + rest.abs() + ref.abs()) + 1e-4).all()
+
+
 def test_steps_with_sparse_reads(need_gpu):
     """A cache that grows by a token a step, its bounds kept up, blocks selected and read, against the plain forms."""
     q, kv, table, lens = make(31, [300, 158, 31], 16, 8, 2, 64, BF16)
@@ -468,6 +537,29 @@ def test_captured_replayed_with_other_contents(need_gpu):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert same(outs[0], one_step(d))
+
+
+def test_first_call_of_a_process_may_be_captured(need_gpu):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from tests.test_gpu_paged_kv import fresh, one_step, same
+s = fresh(40)
+g = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    out = one_step(s)
+g.replay()
+torch.cuda.synchronize()
+assert same(out, one_step(fresh(40)))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-3000:]
 
 
 def test_calls_on_two_streams_at_once(need_gpu):

@@ -82,6 +82,9 @@ def test_attention_refuses_too_many_requests_and_tokens():
         ops.paged_kv_attention(q, kv, table[:, :1].expand(1, 2**27), lens)
     with pytest.raises(ValueError, match="too large"):
         ops.paged_kv_attention(q.expand(64, -1, -1), kv, table[:, :1].expand(64, 2**26 - 1), lens.expand(64))
+    q, kv, table, lens = make(0, [5], 1, 4, 2, 64, torch.bfloat16)
+    with pytest.raises(ValueError, match="too large"):  # 2**31 blocks of one token
+        ops.paged_kv_bounds(kv, table[:, :1].expand(4, 2**29), lens.repeat(4), torch.zeros(kv.shape[1], 2, 2, 64, dtype=kv.dtype))
     with pytest.raises(ValueError, match="a block"):
         ops.paged_kv_evict(torch.zeros(table.shape), table, lens, 4, block_size=65537)
 
@@ -140,3 +143,34 @@ def test_a_query_that_splits_pairs_is_copied(good):
         got = native_kv().whole_pairs(x)
         assert got.data_ptr() % 4 == 0 and got.is_contiguous() and torch.equal(got, q)
     assert native_kv().whole_pairs(q).data_ptr() == q.data_ptr()
+
+
+def test_offloader_saves_what_leaves(monkeypatch):
+    from pcie_pool_b200.adapters.kv_offload import EvictedKV, _EvictsKV
+
+    table = torch.tensor([[7, 3, 9, 4], [5, 6, -1, -1], [1, 2, 8, 0]], dtype=torch.int32)
+    gone = [[3, 9, -1, -1], [-1] * 4, [2, -1, -1, -1]]
+    at = [[1, 2, -1, -1], [-1] * 4, [1, -1, -1, -1]]
+    asked = {}
+
+    def evict(mass, block_table, context_lens, budget, **more):
+        asked.update(more, budget=budget)
+        t = [torch.tensor(x, dtype=torch.int32) for x in (gone, at, [2, 0, 1])]
+        return ops.KVEviction(table, None, None, *t)
+
+    monkeypatch.setattr(ops, "paged_kv_evict", evict)
+
+    class Store(_EvictsKV):
+        calls = []
+
+        def save(self, ids, *host, host_off=0):
+            self.calls.append((ids, host, host_off))
+            return len(ids)
+
+        def prefix_bytes(self, n):
+            return 100 * n
+
+    e, out = Store().evict(None, table, None, 3, "ptr", 4000, block_size=16, host_off=50, recent=2)
+    assert asked == dict(budget=3, block_size=16, sink=1, recent=2)
+    assert Store.calls == [([3, 9], ("ptr", 4000), 50), ([2], ("ptr", 4000), 250)]
+    assert out == [EvictedKV(0, [3, 9], [1, 2], 50, 2), EvictedKV(2, [2], [1], 250, 1)]
