@@ -213,7 +213,7 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
     const T* cache = static_cast<const T*>(a.kv.base) + g * a.kv.head_stride;
 
     float o[DP / 8][4], m[2], l[2];
-    uint32_t q[DP / 16][4];
+    uint32_t q[DP / 16][4] = {};
     const float to_base2 = a.scale * kLog2e;
     int b = request_of(first, n, lo);
     uint32_t end = 0;  // of request b's tiles
@@ -282,15 +282,17 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
         while (first[b + 1] <= (takes ? tile : lo)) ++b;
         end = first[b + 1];
         const T* qp = static_cast<const T*>(a.q.base) + b * a.q.stride + (g * G + row0) * a.q.head_stride;
+        qp += (lane / 4) * a.q.head_stride + (lane & 3) * 2;
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
+        for (int x = 0; x < (PACKED ? 1 : 2); ++x) {
+          const bool on = lane / 4 + 8 * x < rows;
+          const T* at = qp + 8 * x * a.q.head_stride;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = lane / 4 + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
-            q[k][i] = (PACKED && (i & 1)) || row >= rows || d >= D
-                          ? 0u
-                          : *reinterpret_cast<const uint32_t*>(qp + row * a.q.head_stride + d);
+          for (int k = 0; k < DP / 16; ++k) {
+            q[k][x] = on && (D == DP || k * 16 < D) ? *reinterpret_cast<const uint32_t*>(at + k * 16) : 0u;
+            q[k][x + 2] = on && (D == DP || k * 16 + 8 < D) ? *reinterpret_cast<const uint32_t*>(at + k * 16 + 8) : 0u;
           }
+        }
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         m[0] = m[1] = -INFINITY;
@@ -428,23 +430,27 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
           if (row >= rows) continue;
           const int h = g * G + row0 + row;
           const long long at = static_cast<long long>(slot) * w.groups * w.rows + static_cast<long long>(group) * w.rows + row;
-          const float by = sum == 0.f ? 0.f : 1.f / sum;
           if ((lane & 3) == 0) {
             if (whole)
               a.lse[static_cast<long long>(b) * a.q.heads + h] = sum == 0.f ? -INFINITY : (m[x] + lg2(sum)) * kLn2;
             else
               w.part_ml[at] = make_float2(m[x], sum);
           }
+          // (a loop for each: the branch within one loop made a request's end 1 us longer)
+          if (whole) {
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            T* to = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.q.heads + h) * D + (lane & 3) * 2;
 #pragma unroll
-          for (int i = 0; i < DP / 8; ++i) {
-            const int d = i * 8 + (lane & 3) * 2;
-            const float u = PACKED ? o[i][0] + o[i][2] : o[i][2 * x], v = PACKED ? o[i][1] + o[i][3] : o[i][2 * x + 1];
-            if (d < D) {
-              if (whole)
-                *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (static_cast<long long>(b) * a.q.heads + h) * D + d) =
-                    Type<T>::pack(sum == 0.f ? 0.f : u * by, sum == 0.f ? 0.f : v * by);
-              else
-                *reinterpret_cast<float2*>(w.part_o + at * D + d) = make_float2(u, v);
+            for (int i = 0; i < DP / 8; ++i) {
+              const float u = PACKED ? o[i][0] + o[i][2] : o[i][2 * x], v = PACKED ? o[i][1] + o[i][3] : o[i][2 * x + 1];
+              if (D == DP || i * 8 < D) *reinterpret_cast<uint32_t*>(to + i * 8) = Type<T>::pack(sum == 0.f ? 0.f : u * by, sum == 0.f ? 0.f : v * by);
+            }
+          } else {
+            float* to = w.part_o + at * D + (lane & 3) * 2;
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i) {
+              const float u = PACKED ? o[i][0] + o[i][2] : o[i][2 * x], v = PACKED ? o[i][1] + o[i][3] : o[i][2 * x + 1];
+              if (D == DP || i * 8 < D) *reinterpret_cast<float2*>(to + i * 8) = make_float2(u, v);
             }
           }
         }
