@@ -6,8 +6,8 @@
 // Every key and value is read once and used for the G query heads of its key
 // head: 2 G flops a byte, so the cache's bytes bound it, not the arithmetic.  A
 // warp works alone: it streams tiles of 16 tokens of one key head through its
-// own ring of shared memory (cp.async, 16 bytes a lane, a page looked up one
-// tile ahead) and keeps the G x dim result in registers with the running maximum
+// own ring of shared memory (cp.async, 16 bytes a lane, pages looked up 32 blocks
+// ahead) and keeps the G x dim result in registers with the running maximum
 // and sum of the softmax.  No barrier stands in the loop, and tiles of the next
 // request are already on their way while the last one is finished.  Consecutive
 // warps take the key heads of the same tokens, so a page's rows, which lie next
@@ -20,6 +20,15 @@
 // padding).  Weights are multiplied as two numbers of the cache's type, high part and
 // remainder, so the result is as exact as with weights in fp32; up to eight
 // heads, the remainders are the eight rows that the heads leave free and cost nothing.
+//
+// Measured (bf16, 32 heads on 8 key heads of 128, blocks of 16, both kernels, a graph of
+// calls over cold data): 8 x 32768 tokens, 1.07 GB, 163 us, 6.59 TB/s, what a copy
+// reaches; 64 requests of 91 to 8192 tokens, 462 MB, 83 us; 64 x 1024, 268 MB, 52 us;
+// 1 x 16384, 67 MB, 19 us; 1 x 300, 8 us.  What is above the bytes' time is 4 us until
+// the first tiles are asked for (lengths, then pages, each a read from memory), 3 us
+// where a request ends within a range, and 4 us from the last range's end to the
+// join's.  Over a second of such calls the chip is at its power limit and at
+// 1.64 GHz; 8 x 32768 tokens then take 177 to 192 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -42,14 +51,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // Warps of a CTA and tiles in flight of each, by the padded dim: about 192 KiB
-// of shared memory, one CTA to an SM.
+// of shared memory, one CTA to an SM.  (Two tiles of dim 128 in place of three are 13%
+// slower at 64 x 1024 tokens.)
 template <int DP>
 struct Shape {
   static constexpr int kWarps = DP == 256 ? 4 : 8;
   static constexpr int kStages = DP == 64 ? 6 : 3;
   static constexpr int kStageBytes = 2 * kTile * DP * 2;  // K, then V
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  // of a thread: a quarter of the SM's registers is left for a CTA of the join
+  // of a thread: a quarter of the SM's registers is left for a CTA of the join (with 255,
+  // the join starts later: 9.1 us in place of 8.1 for one request of 300 tokens)
   static constexpr int kRegisters = DP == 256 ? 255 : 192;
 };
 
@@ -473,7 +484,7 @@ struct Join {
 // tiles for every head (they lie together) over the heads' totals.  The totals of
 // a request that was cut are taken from its parts, eight lanes for a head, since
 // the join beside it only writes them now; the tiles' sums and the old mass are on
-// their way meanwhile.
+// their way meanwhile.  It adds 2 to 3 us to a call (64 x 1024 tokens: 52 and 55 us).
 constexpr int kMassBlocks = kJoinWarps, kMassHeads = 1024, kMassAhead = 8;
 
 __device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, uint32_t cta) {
@@ -535,7 +546,8 @@ __device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, ui
 // begin, and is the one to work if that is the first cut of its request.  Its warps
 // share `units_each` units, 4 * LANES columns of a query head; LANES lanes take a part
 // and a warp 32 / LANES * kJoinParts parts at a time.  With LANES = 8 that is 160 for a
-// CTA: all parts of a request that lies over all SMs are in flight at once.
+// CTA: all parts of a request that lies over all SMs are in flight at once.  With a CTA
+// for each request and head, 1024 requests of 16 tokens took 96 us in place of 35.
 template <typename T, int LANES, bool MASS>
 __global__ void __launch_bounds__(kJoinWarps * 32, 4)
     attention_join_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w, const __grid_constant__ Join j) {
