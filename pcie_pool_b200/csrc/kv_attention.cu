@@ -698,7 +698,8 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
   Join j;
   const uint32_t items = w.by_cut ? w.most_ranges - 1 : a.req.requests;
   // narrow units while the CTAs fit beside the attention's, else whole rows, and
-  // as many warps for a unit as leave two CTAs to an SM
+  // as many warps for a unit as leave two CTAs to an SM (1 x 16384 tokens: 20.6 us with
+  // narrow units, 24.2 with rows; 8 x 300: 20.3 with 1024 narrow CTAs, 12.6 this way)
   auto join = w.z ? attention_join_kernel<T, 8, true> : attention_join_kernel<T, 8, false>;
   auto share_out = [&](int columns, int64_t most) {
     const int units = a.q.heads * ((a.kv.dim + columns - 1) / columns);

@@ -619,7 +619,8 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const __grid_constant__ 
 }
 
 // By the longest row there can be: few threads with many values each, since what a
-// warp does besides its values costs more than they do.
+// warp does besides its values costs more than they do, but no more places than values
+// (512 x 32 for rows of 8192 makes the selection 3 us longer than 512 x 16).
 template <typename Launch>
 void for_width(int width, Launch launch) {
   using std::integral_constant;
