@@ -226,12 +226,19 @@ def kv_layout(kv) -> KVLayout:
     return KVLayout(1, 0, kv.stride(0) * es, kv.stride(0) * es, shape[0])
 
 
+def check_block_ids(ids: np.ndarray, num_blocks: int) -> None:
+    """ValueError for ids outside [0, num_blocks): their addresses would lie outside the cache."""
+    if ids.size and (int(ids.min()) < 0 or int(ids.max()) >= num_blocks):
+        raise ValueError(f"block id outside the kv cache of {num_blocks} blocks")
+
+
 def block_table_units(kv_caches: Iterable, block_ids: Iterable[int]) -> tuple[np.ndarray, int]:
     """Device address of every (layer, lane, block) unit of a request in the
     CPU backing order [layer][lane][index] -> (uint64 addresses, unit bytes).
 
     The landing kernel scatters a host-contiguous chunk of units through this
     table (paged-KV reload) and the push kernel gathers through it (offload).
+    Both trust the addresses, so an id that is no block of a cache is refused here.
     """
     ids = np.asarray(list(block_ids), dtype=np.int64)
     out, unit = [], None
@@ -241,6 +248,7 @@ def block_table_units(kv_caches: Iterable, block_ids: Iterable[int]) -> tuple[np
             unit = lay.unit_bytes
         elif lay.unit_bytes != unit:
             raise ValueError("all layers must share one block size")
+        check_block_ids(ids, lay.num_blocks)
         base = int(kv.data_ptr())
         for lane in range(lay.lanes):
             out.append(base + lane * lay.lane_stride + ids * lay.block_stride)
@@ -256,6 +264,6 @@ make_layer_block_refs_from_ids = make_vllm_layer_block_refs_from_ids
 make_layer_range_refs_from_ids = make_vllm_layer_range_refs_from_ids
 
 __all__ = ["VllmKVBlockRef", "VllmKVGroup", "VllmKVSlotAdapter", "block_bytes_from_vllm_kv_tensor",
-           "KVLayout", "block_table_units", "contiguous_runs", "kv_layout", "make_vllm_block_refs_from_ids",
+           "KVLayout", "block_table_units", "check_block_ids", "contiguous_runs", "kv_layout", "make_vllm_block_refs_from_ids",
            "make_vllm_layer_block_refs_from_ids", "make_vllm_layer_groups_from_kv_caches",
            "make_vllm_layer_range_refs_from_ids", "vllm_block_name"]

@@ -71,28 +71,33 @@ def scatter_units(src, addrs, unit_bytes: int):
                                _stream(src))
 
 
-def paged_kv_gather(kv, block_ids, out=None):
-    """Gather K/V blocks of one vLLM layer cache ``[2, num_blocks, ...]`` into a
-    contiguous buffer laid out [K blocks in order, V blocks in order]."""
-    torch = _torch()
+def _paged_kv_units(kv, block_ids):
+    """(int64 CUDA tensor of the unit addresses [K blocks in order, V blocks in order], unit bytes)."""
+    from ..adapters.vllm import check_block_ids
+
+    ids = np.asarray(block_ids, dtype=np.int64)
+    check_block_ids(ids, kv.shape[1])
     blk = kv.stride(1) * kv.element_size()
     lane = kv.stride(0) * kv.element_size()
-    ids = np.asarray(block_ids, dtype=np.int64)
     offs = np.concatenate([ids * blk, lane + ids * blk])
-    addrs = torch.as_tensor(offs + kv.data_ptr(), device=kv.device)
+    return _torch().as_tensor(offs + kv.data_ptr(), device=kv.device), blk
+
+
+def paged_kv_gather(kv, block_ids, out=None):
+    """Gather K/V blocks of one vLLM layer cache ``[2, num_blocks, ...]`` into a
+    contiguous buffer laid out [K blocks in order, V blocks in order].  Ids that
+    are no block of the cache raise ``ValueError``."""
+    torch = _torch()
+    addrs, blk = _paged_kv_units(kv, block_ids)
     if out is None:
-        out = torch.empty(offs.size * blk, dtype=torch.uint8, device=kv.device)
+        out = torch.empty(addrs.numel() * blk, dtype=torch.uint8, device=kv.device)
     gather_units(addrs, blk, out)
     return out
 
 
 def paged_kv_scatter(kv, block_ids, src):
-    torch = _torch()
-    blk = kv.stride(1) * kv.element_size()
-    lane = kv.stride(0) * kv.element_size()
-    ids = np.asarray(block_ids, dtype=np.int64)
-    offs = np.concatenate([ids * blk, lane + ids * blk])
-    addrs = torch.as_tensor(offs + kv.data_ptr(), device=kv.device)
+    """The reverse of ``paged_kv_gather``."""
+    addrs, blk = _paged_kv_units(kv, block_ids)
     scatter_units(src, addrs, blk)
 
 

@@ -1,0 +1,55 @@
+"""Pages of the paged KV cache on the host's side, on CPU: ids that are no page of the cache, pages that requests
+share, and the room that an eviction needs."""
+
+import pytest
+import torch
+
+from pcie_pool_b200 import ops
+from pcie_pool_b200.adapters import PagedKVOffloader
+from pcie_pool_b200.adapters.vllm import block_table_units
+
+PAGES = 8
+
+
+class Engine:
+    """Stands for the pool engine: no transfer may reach it."""
+
+    def run(self, *args, **more):
+        raise AssertionError("a transfer was started")
+
+
+def cache(pages_first=False):
+    shape = (PAGES, 2, 16, 2, 64) if pages_first else (2, PAGES, 16, 2, 64)
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+# ---- ids outside the cache ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("pages_first", [False, True])
+@pytest.mark.parametrize("ids", [[PAGES], [3, 1000], [-1], [0, -7, 2], [2**31 - 1]])
+def test_ids_outside_the_cache_get_no_address(pages_first, ids):
+    kvs = [cache(pages_first) for _ in range(2)]
+    with pytest.raises(ValueError, match="outside the kv cache"):
+        block_table_units(kvs, ids)
+    store = PagedKVOffloader(Engine(), kvs, target=0, sync_stream=False)
+    with pytest.raises(ValueError, match="outside the kv cache"):
+        store.save(ids, 4096, 1 << 30)
+    with pytest.raises(ValueError, match="outside the kv cache"):
+        store.restore(ids, 4096, 1 << 30)
+
+
+@pytest.mark.parametrize("ids", [[PAGES], [-1, 0]])
+def test_gather_and_scatter_refuse_ids_outside_the_cache(ids):
+    with pytest.raises(ValueError, match="outside the kv cache"):
+        ops.paged_kv_gather(cache(), ids)
+    with pytest.raises(ValueError, match="outside the kv cache"):
+        ops.paged_kv_scatter(cache(), ids, torch.zeros(1 << 16, dtype=torch.uint8))
+
+
+def test_ids_of_the_cache_are_taken():
+    kvs = [cache(), cache()]
+    addrs, unit = block_table_units(kvs, [PAGES - 1, 0])
+    last = kvs[1].data_ptr() + kvs[1].numel() * 2 - unit
+    assert last in addrs.tolist() and int(addrs.min()) >= min(kv.data_ptr() for kv in kvs)
+    assert block_table_units(kvs, [])[0].size == 0
