@@ -212,6 +212,14 @@ class KVLayout:
     num_blocks: int
 
 
+def check_planes(lane_stride: int, block_stride: int, num_blocks: int) -> None:
+    """ValueError for a ``[2, num_blocks, ...]`` view whose K and V are not planes of their own: its block
+    stride spans both lanes, so a unit would cover its neighbour's keys and the last one end past the cache."""
+    if num_blocks and lane_stride < num_blocks * block_stride:
+        raise ValueError("K and V of a block lie next to each other in this KV tensor: "
+                         "pass it as [num_blocks, 2, ...], not as a [2, num_blocks, ...] view")
+
+
 def kv_layout(kv) -> KVLayout:
     """Layout of a vLLM KV cache tensor.  ``[2, num_blocks, ...]`` (K and V
     planes, e.g. the FlashAttention backend) has two units per block;
@@ -220,6 +228,7 @@ def kv_layout(kv) -> KVLayout:
     es = kv.element_size()
     shape = tuple(int(d) for d in kv.shape)
     if len(shape) >= 3 and shape[0] == 2 and shape[1] != 2:
+        check_planes(kv.stride(0), kv.stride(1), shape[1])
         return KVLayout(2, kv.stride(0) * es, kv.stride(1) * es, kv.stride(1) * es, shape[1])
     if len(shape) < 2:
         raise ValueError("vLLM KV tensor must have at least two dimensions")

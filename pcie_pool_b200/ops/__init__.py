@@ -73,9 +73,10 @@ def scatter_units(src, addrs, unit_bytes: int):
 
 def _paged_kv_units(kv, block_ids):
     """(int64 CUDA tensor of the unit addresses [K blocks in order, V blocks in order], unit bytes)."""
-    from ..adapters.vllm import check_block_ids
+    from ..adapters.vllm import check_block_ids, check_planes
 
     ids = np.asarray(block_ids, dtype=np.int64)
+    check_planes(kv.stride(0), kv.stride(1), kv.shape[1])
     check_block_ids(ids, kv.shape[1])
     blk = kv.stride(1) * kv.element_size()
     lane = kv.stride(0) * kv.element_size()
@@ -85,8 +86,9 @@ def _paged_kv_units(kv, block_ids):
 
 def paged_kv_gather(kv, block_ids, out=None):
     """Gather K/V blocks of one vLLM layer cache ``[2, num_blocks, ...]`` into a
-    contiguous buffer laid out [K blocks in order, V blocks in order].  Ids that
-    are no block of the cache raise ``ValueError``."""
+    contiguous buffer laid out [K blocks in order, V blocks in order].  K and V
+    are planes of their own; other views, and ids that are no block of the cache,
+    raise ``ValueError``."""
     torch = _torch()
     addrs, blk = _paged_kv_units(kv, block_ids)
     if out is None:

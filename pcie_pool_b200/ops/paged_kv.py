@@ -2,10 +2,10 @@
 request, the key bounds of the cache's pages, the blocks that sparse attention
 reads, and the blocks that may leave the GPU.
 
-The cache is the layer tensor that ``paged_kv_gather`` takes: ``[2, pages,
-block, kv_heads, dim]``, K then V, in any strides that are multiples of 16 bytes
-with a contiguous last dimension; a ``[pages, 2, ...]`` cache is passed as
-``kv.transpose(0, 1)``.  Request ``b`` holds ``context_lens[b]`` tokens, block
+The cache of a layer is ``[2, pages, block, kv_heads, dim]``, K then V, in any
+strides that are multiples of 16 bytes with a contiguous last dimension; a
+``[pages, 2, ...]`` cache is passed as ``kv.transpose(0, 1)`` (to these operators
+only: the offloaders take it as it is).  Request ``b`` holds ``context_lens[b]`` tokens, block
 ``j`` of it in page ``block_table[b, j]``.  A table entry that is no page
 (negative, or ``>= pages``) is a block that is not resident -- offloaded, say --
 and its tokens are left out.  Lengths and tables are read on the device when the

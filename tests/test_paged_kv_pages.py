@@ -53,3 +53,27 @@ def test_ids_of_the_cache_are_taken():
     last = kvs[1].data_ptr() + kvs[1].numel() * 2 - unit
     assert last in addrs.tolist() and int(addrs.min()) >= min(kv.data_ptr() for kv in kvs)
     assert block_table_units(kvs, [])[0].size == 0
+
+
+# ---- views whose K and V lie next to each other ------------------------------------------------
+
+
+def test_a_transposed_cache_is_no_cache_of_planes():
+    """Its units would be two lanes long: the last one ends past the cache, the others cover the next block's keys."""
+    view = cache(pages_first=True).transpose(0, 1)
+    with pytest.raises(ValueError, match="next to each other"):
+        block_table_units([view], [0])
+    with pytest.raises(ValueError, match="next to each other"):
+        PagedKVOffloader(Engine(), [view], target=0)
+    with pytest.raises(ValueError, match="next to each other"):
+        ops.paged_kv_gather(view, [0])
+    with pytest.raises(ValueError, match="next to each other"):
+        ops.paged_kv_scatter(view, [0], torch.zeros(1 << 16, dtype=torch.uint8))
+
+
+def test_planes_of_any_inner_order_are_taken():
+    heads = torch.zeros(2, PAGES, 2, 16, 64, dtype=torch.bfloat16).transpose(2, 3)
+    apart = torch.zeros(2, PAGES + 3, 16, 2, 64, dtype=torch.bfloat16)[:, 2: 2 + PAGES]
+    for kv in (heads, apart):
+        addrs, unit = block_table_units([kv], range(PAGES))
+        assert unit == 16 * 2 * 64 * 2 and addrs[-1] == kv.data_ptr() + kv.stride(0) * 2 + (PAGES - 1) * unit
