@@ -58,6 +58,8 @@ class EvictedKV:
 class _EvictsKV:
     """Eviction by accumulated attention weight, for what has ``save`` and ``prefix_bytes``."""
 
+    num_blocks: int | None = None  # pages of the caches: table entries from there on are not resident
+
     def evict(self, mass, block_table, context_lens, budget: int, *host, block_size: int, host_off: int = 0,
               sink: int = 1, recent: int = 1):
         """Cut every request to ``budget`` blocks (``ops.paged_kv_evict``: ``mass`` is what
@@ -68,7 +70,9 @@ class _EvictsKV:
         and ``restore(pages, *host, host_off=...)`` brings a request's evicted blocks back."""
         from ..ops import paged_kv_evict
 
-        e = paged_kv_evict(mass, block_table, context_lens, budget, block_size=block_size, sink=sink, recent=recent)
+        known = {} if self.num_blocks is None else {"pages": self.num_blocks}
+        e = paged_kv_evict(mass, block_table, context_lens, budget, block_size=block_size, sink=sink, recent=recent,
+                           **known)
         counts = e.evicted_count.tolist()
         widest = max(counts, default=0)
         pages, places = e.evicted_blocks[:, :widest].tolist(), e.evicted_index[:, :widest].tolist()
@@ -99,6 +103,7 @@ class PagedKVOffloader(_EvictsKV):
         lay = kv_layout(self.kv_caches[0])
         self.unit_bytes = lay.unit_bytes
         self.units_per_block = lay.lanes * len(self.kv_caches)
+        self.num_blocks = min(kv_layout(kv).num_blocks for kv in self.kv_caches)
 
     def prefix_bytes(self, block_count: int) -> int:
         return int(block_count) * self.units_per_block * self.unit_bytes
@@ -218,6 +223,7 @@ class DaemonKVOffloader(_EvictsKV):
         lay = kv_layout(self.kv_caches[0])
         self.unit_bytes = lay.unit_bytes
         self.units_per_block = lay.lanes * len(self.kv_caches)
+        self.num_blocks = min(kv_layout(kv).num_blocks for kv in self.kv_caches)
         self.units_per_chunk = int(units_per_chunk)
         self.prefix = str(prefix)
         self.ctas_per_lane = int(ctas_per_lane)

@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const __grid_constant__ 
   const float* mass = e.mass + b * e.mass_stride;
   const int* table = e.req.table + b * e.req.table_stride;
   const long long at0 = static_cast<long long>(b) * width;
-  Keys row({mass, table, INT_MAX, n, e.sink, e.recent}, n, shared);
+  Keys row({mass, table, e.pages, n, e.sink, e.recent}, n, shared);
   const Border border = row.border(e.budget);
   int tokens = 0;
   row.template emit<true>(

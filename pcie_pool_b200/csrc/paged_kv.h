@@ -81,6 +81,7 @@ struct KvEvict {
   KvRequests req;
   const float* mass = nullptr;
   int64_t mass_stride = 0;
+  int pages = 0;  // table entries outside [0, pages) are dropped
   int block = 0, budget = 0, sink = 0, recent = 0;
   int* new_table = nullptr;    // [requests, width]
   int* new_lens = nullptr;     // [requests]

@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <limits>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -214,7 +215,7 @@ Tensor kv_select(const Tensor& given, const Tensor& bounds, const Tensor& table,
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> kv_evict(const Tensor& mass, const Tensor& table,
                                                                     const Tensor& lens, const py::object& budget,
                                                                     const py::object& block, const py::object& sink,
-                                                                    const py::object& recent) {
+                                                                    const py::object& recent, const py::object& pages) {
   need(mass.scalar_type() == at::kFloat && mass.sizes() == table.sizes(), "mass must be fp32 in block_table's shape");
   KvEvict e;
   e.block = whole(block, 1, "block_size must be an integer >= 1");
@@ -226,6 +227,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> kv_evict(const Tensor
   e.sink = whole(sink, 0, "sink must be an integer >= 0");
   e.recent = whole(recent, 1, "recent must be an integer >= 1");
   need(int64_t(e.sink) + e.recent <= e.budget, "budget must be at least sink + recent");
+  e.pages = !pages.is_none() ? whole(pages, 0, "pages must be an integer >= 0") : std::numeric_limits<int>::max();
   const cudaStream_t stream = stream_of({&mass});
   const at::IntArrayRef rows = table.sizes();
   const at::Device device = mass.device();

@@ -99,15 +99,19 @@ class KVEviction(NamedTuple):
     evicted_count: object   # int32 [requests]
 
 
-def paged_kv_evict(mass, block_table, context_lens, budget, *, block_size, sink=1, recent=1) -> KVEviction:
+def paged_kv_evict(mass, block_table, context_lens, budget, *, block_size, sink=1, recent=1,
+                   pages=None) -> KVEviction:
     """Cut every request to at most ``budget`` blocks: the first ``sink`` and the last
     ``recent`` stay, the others by accumulated attention weight (``mass`` of
     ``paged_kv_attention``), ties to the lowest index; mass that is not a number
     ranks lowest.  ``recent`` is at least 1, so the block that is being filled
-    stays the last.  Negative table entries (blocks that are not resident) are
-    dropped and not listed.  The inputs are left as they were.
+    stays the last.  Blocks that are not resident take no place in the
+    budget, are dropped and not listed: negative table entries, and with ``pages``,
+    the cache's number of pages, entries from there on too (without it every other
+    entry is taken for a page).  The inputs are left as they were.
     """
-    return KVEviction(*native_kv().evict(mass, block_table, context_lens, budget, block_size, sink, recent))
+    return KVEviction(*native_kv().evict(mass, block_table, context_lens, budget, block_size, sink, recent,
+                                          pages))
 
 
 __all__ = ["KVEviction", "paged_kv_attention", "paged_kv_bounds", "paged_kv_evict", "paged_kv_select"]

@@ -1,0 +1,68 @@
+"""GPU tests of the paged-KV operators at the edges of what they take: entries that are no page, counts near their
+limits, weights far below the leading one, values that are not finite, memory that arguments share."""
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from pcie_pool_b200 import ops  # noqa: E402
+from tests.paged_kv_cases import best, make, to_gpu  # noqa: E402
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+# ---- eviction: entries that are no page of the cache -----------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [13, 700, 9000])
+def test_evict_drops_entries_that_are_no_page(need_gpu, n):
+    """They take no place in the budget, though they hold the most mass or stand first or last."""
+    pages, budget = 2 * n, n // 2
+    g = torch.Generator().manual_seed(n)
+    table = torch.randperm(pages, generator=g)[:n].to(torch.int32)[None]
+    mass = torch.rand(1, n, generator=g)
+    bad = torch.tensor([0, 3, 4, n - 1])
+    table[0, bad] = torch.tensor([pages, 2**31 - 1, -1, pages + 7], dtype=torch.int32)
+    mass[0, bad] = 100.0
+    can = [0 <= int(p) < pages for p in table[0]]
+    stay = best(mass[0].tolist(), can, budget, 2, 3)
+    gone = [j for j in range(n) if can[j] and j not in set(stay)]
+    e = ops.paged_kv_evict(mass.cuda(), table.cuda(), torch.tensor([16 * n - 5], dtype=torch.int32).cuda(), budget,
+                           block_size=16, sink=2, recent=3, pages=pages)
+    assert e.block_table[0].tolist() == table[0, stay].tolist() + [-1] * (n - len(stay))
+    assert e.evicted_blocks[0].tolist() == table[0, gone].tolist() + [-1] * (n - len(gone))
+    assert e.evicted_index[0].tolist() == gone + [-1] * (n - len(gone))
+    assert e.evicted_count.tolist() == [len(gone)] and e.context_lens.tolist() == [16 * len(stay)]
+
+
+def test_offloader_evicts_around_entries_that_are_no_page(need_gpu):
+    """A table with an entry past the cache: what is saved is the evicted pages' own, read back from the host."""
+    from pcie_pool_b200.adapters import PagedKVOffloader
+    from pcie_pool_b200.parallel.engine import PoolEngine
+    from pcie_pool_b200.utils.host_memory import PinnedHostBuffer
+
+    pages = 24
+    g = torch.Generator().manual_seed(1)
+    kv = torch.randn(2, pages, 16, 2, 64, generator=g).to(BF16).cuda()
+    table = torch.randperm(pages, generator=g)[:12].to(torch.int32)[None]
+    table[0, 2], table[0, 5] = pages, pages + 1000
+    mass = torch.rand(1, 12, generator=g)
+    mass[0, [2, 5]] = 50.0
+    host = PinnedHostBuffer(1 << 20)
+    try:
+        store = PagedKVOffloader(PoolEngine([0], slot_bytes=1 << 20, slots=3, timeout_s=10.0), [kv], target=0)
+        e, gone = store.evict(mass.cuda(), table.cuda(), torch.tensor([12 * 16], dtype=torch.int32).cuda(), 4, host.ptr, 1 << 20,
+                              block_size=16)
+        assert len(gone) == 1 and len(gone[0].blocks) == 6 and all(0 <= p < pages for p in gone[0].blocks)
+        assert set(e.block_table[0, :4].tolist()) | set(gone[0].blocks) == {int(p) for p in table[0] if p < pages}
+        saved = kv[:, gone[0].blocks].clone()
+        kv.zero_()
+        store.restore(gone[0].blocks, host.ptr, 1 << 20, host_off=gone[0].host_off)
+        torch.cuda.synchronize()
+        assert torch.equal(kv[:, gone[0].blocks], saved)
+    finally:
+        host.release()

@@ -77,3 +77,30 @@ def test_planes_of_any_inner_order_are_taken():
     for kv in (heads, apart):
         addrs, unit = block_table_units([kv], range(PAGES))
         assert unit == 16 * 2 * 64 * 2 and addrs[-1] == kv.data_ptr() + kv.stride(0) * 2 + (PAGES - 1) * unit
+
+
+# ---- eviction and the cache's number of pages ---------------------------------------------------------
+
+
+def test_offloaders_tell_the_eviction_how_many_pages_there_are(monkeypatch):
+    asked = []
+
+    def evict(*args, **more):
+        asked.append(more)
+        none = torch.full((1, 2), -1, dtype=torch.int32)
+        return ops.KVEviction(none, None, None, none, none, torch.zeros(1, dtype=torch.int32))
+
+    monkeypatch.setattr(ops, "paged_kv_evict", evict)
+    for kvs in ([cache(), cache()], [cache(pages_first=True)]):
+        PagedKVOffloader(Engine(), kvs, target=0).evict(None, None, None, 3, 4096, 1 << 20, block_size=16)
+    assert [a["pages"] for a in asked] == [PAGES, PAGES]
+
+
+def test_evict_refuses_numbers_of_pages_that_are_none():
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    lens = torch.tensor([50], dtype=torch.int32)
+    for pages in (-1, 8.0, True, 2**31):
+        with pytest.raises(ValueError, match="pages must be"):
+            ops.paged_kv_evict(torch.zeros(1, 4), table, lens, 3, block_size=16, pages=pages)
+    with pytest.raises(ValueError, match="CUDA device"):
+        ops.paged_kv_evict(torch.zeros(1, 4), table, lens, 3, block_size=16, pages=8)
