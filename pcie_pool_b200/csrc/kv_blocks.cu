@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
   Keys row({score, table, s.pages, n, s.sink, s.recent}, n, shared);
   const Border e = row.border(s.keep);
   row.template emit<false>(e, [&](int j, int at) { out[at] = j; }, [](int, int) {});
-  for (int j = row.taken + threadIdx.x; j < s.keep; j += THREADS) out[j] = -1;
+  // (unsigned: keep may be 2^31 - 1, where a step of an int would wrap around)
+  for (unsigned j = row.taken + threadIdx.x; j < static_cast<unsigned>(s.keep); j += THREADS) out[j] = -1;
 }
 
 template <int THREADS, int ITEMS>

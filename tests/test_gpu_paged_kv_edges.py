@@ -66,3 +66,17 @@ def test_offloader_evicts_around_entries_that_are_no_page(need_gpu):
         assert torch.equal(kv[:, gone[0].blocks], saved)
     finally:
         host.release()
+
+
+# ---- selection ----------------------------------------------------------------------------------------
+
+
+def test_select_of_the_most_blocks_there_can_be(need_gpu):
+    """keep = 2**31 - 1: the places behind the row are filled to the last, and nothing before the row."""
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    q, kv, table, lens = make(70, [40], 16, 2, 1, 8, BF16)
+    bounds = torch.zeros(kv.shape[1], 1, 2, 8, dtype=BF16, device="cuda")
+    out = ops.paged_kv_select(q.cuda(), bounds, table.cuda(), lens.cuda(), 2**31 - 1, block_size=16)
+    assert out.shape == (1, 1, 2**31 - 1) and out[0, 0, :3].tolist() == [0, 1, 2]
+    assert all((part == -1).all() for part in out[0, 0, 3:].split(1 << 28))
