@@ -198,6 +198,10 @@ Tensor kv_select(const Tensor& given, const Tensor& bounds, const Tensor& table,
   s.block = whole(block, 1, "block_size must be an integer >= 1");
   s.req = requests_of(table, lens, bounds.device(), s.block);
   const Tensor q = query_of(given, bounds.device(), bounds.scalar_type(), dim, s.kv_heads, s.req.requests, s.q);
+  // a CTA of the selection has a request's key head, a unit of the scores 8 blocks of one
+  const int64_t rows = int64_t(s.req.requests) * s.kv_heads, units = (int64_t(s.req.width) + 7) / 8 * s.kv_heads;
+  need(rows < kInt && units < kInt - kMaxDim && (units / 8 + 1) * s.req.requests < kInt,
+       "too many key heads: at most 2**31 rows of requests and key heads, and 2**34 scores");
   s.keep = whole(keep, 1, "keep must be an integer >= 1");
   s.sink = whole(sink, 0, "sink must be an integer >= 0");
   s.recent = whole(recent, 0, "recent must be an integer >= 0");

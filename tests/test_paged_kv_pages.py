@@ -104,3 +104,26 @@ def test_evict_refuses_numbers_of_pages_that_are_none():
             ops.paged_kv_evict(torch.zeros(1, 4), table, lens, 3, block_size=16, pages=pages)
     with pytest.raises(ValueError, match="CUDA device"):
         ops.paged_kv_evict(torch.zeros(1, 4), table, lens, 3, block_size=16, pages=8)
+
+
+# ---- numbers that 32 bits do not hold ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("requests,kv_heads,width", [(4096, 2**20, 1), (4096, 2**19, 1), (4095, 2**20 + 1, 4), (1, 2**20, 2**15),
+                                                     (4096, 2**12, 2**13)])
+def test_select_refuses_more_rows_than_a_grid_holds(requests, kv_heads, width):
+    """4096 requests of 2**20 key heads were 2**32 rows, 0 in 32 bits: nothing was written to the result."""
+    q = torch.zeros(1, 1, 8, dtype=torch.bfloat16).expand(requests, kv_heads, 8)
+    bounds = torch.zeros(0, kv_heads, 2, 8, dtype=torch.bfloat16)
+    table = torch.zeros(1, 1, dtype=torch.int32).expand(requests, width)
+    table = table if width == 1 else torch.zeros(1, width, dtype=torch.int32).expand(requests, width)
+    with pytest.raises(ValueError, match="too many key heads"):
+        ops.paged_kv_select(q, bounds, table, torch.zeros(requests, dtype=torch.int32), 1, block_size=16, recent=0)
+
+
+def test_select_takes_many_key_heads():
+    q = torch.zeros(1, 1, 8, dtype=torch.bfloat16).expand(2047, 2**20, 8)
+    bounds = torch.zeros(0, 2**20, 2, 8, dtype=torch.bfloat16)
+    table = torch.zeros(1, 1, dtype=torch.int32).expand(2047, 1)
+    with pytest.raises(ValueError, match="CUDA device"):
+        ops.paged_kv_select(q, bounds, table, torch.zeros(2047, dtype=torch.int32), 1, block_size=16, recent=0)
