@@ -18,7 +18,12 @@
 // cost the same whether 1 or 16 heads use them, and at 16 tokens a step the tensor
 // pipe is far from its limit (tcgen05's 128 rows would be 4 or 8 heads and
 // padding).  Weights are multiplied as two numbers of the cache's type, high part and
-// remainder, so the result is as exact as with weights in fp32; up to eight
+// remainder: 16 of their 24 bits in bf16, 22 in fp16, far below the result's own 8 and
+// 11 (of 8 x 32768 tokens in bf16, 1.9 results in a thousand are not the nearest to 64
+// bits; with all 24 bits it is 0.6).  Their sum, the log-sums and the mass take them
+// whole.  fp16 ends at 2^-24,
+// so there the weights, at most 1, are multiplied by 2^15 and the result is divided by it:
+// what is lost of a weight beside the leading one is 2^-40 of that, not 2^-25.  Up to eight
 // heads, the remainders are the eight rows that the heads leave free and cost nothing.
 //
 // Measured (bf16, 32 heads on 8 key heads of 128, blocks of 16, both kernels, a graph of
@@ -108,6 +113,7 @@ struct Type;
 
 template <>
 struct Type<__nv_bfloat16> {
+  static constexpr float kLift = 1.f;  // what weights are multiplied by before they are split
   static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -125,6 +131,7 @@ struct Type<__nv_bfloat16> {
 
 template <>
 struct Type<__half> {
+  static constexpr float kLift = 0x1p15f;
   static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -140,9 +147,11 @@ struct Type<__half> {
   }
 };
 
-// High part of two weights and what it leaves, as pairs.
+// High part of two lifted weights and what it leaves, as pairs.
 template <typename T>
 __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  x *= Type<T>::kLift;
+  y *= Type<T>::kLift;
   hi = Type<T>::pack(x, y);
   const float2 h = Type<T>::unpack(hi);
   lo = Type<T>::pack(x - h.x, y - h.y);
@@ -449,7 +458,7 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
           }
           // (a loop for each: the branch within one loop made a request's end 1 us longer)
           if (whole) {
-            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            const float by = sum == 0.f ? 0.f : 1.f / Type<T>::kLift / sum;
             T* to = static_cast<T*>(a.out) + (static_cast<long long>(b) * a.q.heads + h) * D + (lane & 3) * 2;
 #pragma unroll
             for (int i = 0; i < DP / 8; ++i) {
@@ -461,7 +470,8 @@ __global__ void __maxnreg__(Shape<DP>::kRegisters)
 #pragma unroll
             for (int i = 0; i < DP / 8; ++i) {
               const float u = PACKED ? o[i][0] + o[i][2] : o[i][2 * x], v = PACKED ? o[i][1] + o[i][3] : o[i][2 * x + 1];
-              if (D == DP || i * 8 < D) *reinterpret_cast<float2*>(to + i * 8) = make_float2(u, v);
+              if (D == DP || i * 8 < D)
+                *reinterpret_cast<float2*>(to + i * 8) = make_float2(u * (1.f / Type<T>::kLift), v * (1.f / Type<T>::kLift));
             }
           }
         }

@@ -80,3 +80,52 @@ def test_select_of_the_most_blocks_there_can_be(need_gpu):
     out = ops.paged_kv_select(q.cuda(), bounds, table.cuda(), lens.cuda(), 2**31 - 1, block_size=16)
     assert out.shape == (1, 1, 2**31 - 1) and out[0, 0, :3].tolist() == [0, 1, 2]
     assert all((part == -1).all() for part in out[0, 0, 3:].split(1 << 28))
+
+
+# ---- weights far below the leading one --------------------------------------------------------------------
+
+
+def check_attention(q, kv, table, lens, out, lse, **more):
+    from tests.test_gpu_paged_kv import check_attention as check
+
+    return check(q, kv, table, lens, out, lse, **more)
+
+
+def with_a_leading_token(dtype, heads, kv_heads, dim, tokens, gap, where, seed):
+    """One token `gap` nats above the others, with values a thousand times smaller: what the others give is the result."""
+    q, kv, table, lens = make(seed, [tokens], 16, heads, kv_heads, dim, dtype)
+    q[..., 0], q[..., 1:] = 1.0, 0.0
+    kv[0, ..., 0] = kv[0, ..., 0].abs().clamp(max=0.5)
+    at = (table[0, where // 16], where % 16)
+    kv[0][at][:, 0] = gap
+    kv[1] = kv[1].abs() + 0.5
+    kv[1][at] = kv[1][at] / 1024
+    return q, kv, table, lens
+
+
+@pytest.mark.parametrize("gap", [8.0, 12.0, 14.0, 16.0, 18.0, 20.0])
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,where", [
+    (600, 600, 8, 800, 0), (600, 600, 8, 800, 400), (5400, 600, 8, 320, 0),  # a range holds all tokens; heads alone, and nine to a key head
+    (300, 300, 256, 320, 7),
+    (4, 1, 64, 800, 3), (18, 1, 128, 800, 3)])                               # many ranges, joined
+def test_small_weights_are_not_lost_beside_a_leading_one(need_gpu, heads, kv_heads, dim, tokens, where, gap):
+    q, kv, table, lens = with_a_leading_token(FP16, heads, kv_heads, dim, tokens, gap, where, 71)
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), scale=1.0, return_lse=True)
+    check_attention(q, kv, table, lens, out, lse, scale=1.0)
+
+
+@pytest.mark.parametrize("gap", [8.0, 40.0, 80.0])
+def test_small_weights_in_bf16(need_gpu, gap):
+    q, kv, table, lens = with_a_leading_token(BF16, 600, 600, 8, 800, gap, 400, 72)
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), scale=1.0, return_lse=True)
+    check_attention(q, kv, table, lens, out, lse, scale=1.0)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(600, 600), (5400, 600)])
+def test_large_values_in_fp16(need_gpu, heads, kv_heads):
+    """Values at the type's end: what is summed is larger than they are by the weights' scale and the tokens' number."""
+    q, kv, table, lens = make(73, [320], 16, heads, kv_heads, 8, FP16)
+    kv[1] = torch.where(kv[1] > 0, 65504.0, -65504.0).to(FP16).where(~torch.isnan(kv[1]), kv[1])
+    kv[1][..., 0] = kv[1][..., 0].abs()
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), scale=0.25, return_lse=True)
+    check_attention(q, kv, table, lens, out, lse, scale=0.25)
