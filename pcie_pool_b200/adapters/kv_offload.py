@@ -60,6 +60,10 @@ class _EvictsKV:
 
     num_blocks: int | None = None  # pages of the caches: table entries from there on are not resident
 
+    def _host_bytes(self, *host) -> int | None:
+        """Bytes of the host region, if they are known."""
+        return None
+
     def evict(self, mass, block_table, context_lens, budget: int, *host, block_size: int, host_off: int = 0,
               sink: int = 1, recent: int = 1):
         """Cut every request to ``budget`` blocks (``ops.paged_kv_evict``: ``mass`` is what
@@ -67,13 +71,20 @@ class _EvictsKV:
         transfer for each request that loses any, one behind the other from ``host_off``; ``host``
         is what ``save`` takes.  Returns (``KVEviction``, list of ``EvictedKV``): the requests go
         on with the eviction's table, lengths and mass, the pages of ``EvictedKV.blocks`` are free,
-        and ``restore(pages, *host, host_off=...)`` brings a request's evicted blocks back."""
+        and ``restore(pages, *host, host_off=...)`` brings a request's evicted blocks back.
+
+        The room for all of them is checked before the first transfer (``ValueError``). The inputs
+        and the cache's pages are left as they were, so after an error, of a transfer too, the caller
+        still has all that it had."""
         from ..ops import paged_kv_evict
 
         known = {} if self.num_blocks is None else {"pages": self.num_blocks}
         e = paged_kv_evict(mass, block_table, context_lens, budget, block_size=block_size, sink=sink, recent=recent,
                            **known)
         counts = e.evicted_count.tolist()
+        room, need = self._host_bytes(*host), sum(self.prefix_bytes(n) for n in counts)
+        if host_off < 0 or (room is not None and need and host_off + need > room):
+            raise ValueError(f"the {need} bytes of the blocks that leave do not fit the host region from offset {host_off} on")
         widest = max(counts, default=0)
         pages, places = e.evicted_blocks[:, :widest].tolist(), e.evicted_index[:, :widest].tolist()
         out = []
@@ -107,6 +118,9 @@ class PagedKVOffloader(_EvictsKV):
 
     def prefix_bytes(self, block_count: int) -> int:
         return int(block_count) * self.units_per_block * self.unit_bytes
+
+    def _host_bytes(self, host_ptr: int, host_bytes: int) -> int:
+        return int(host_bytes)
 
     def _segments(self, nunits: int, host_off: int, span_blocks: int | None, nblocks: int):
         return kv_segments(nunits, host_off, span_blocks, nblocks, self.unit_bytes)
@@ -281,6 +295,9 @@ class DaemonKVOffloader(_EvictsKV):
         return bid
 
     # ---- transfers --------------------------------------------------------------------
+    def _host_bytes(self, host) -> int:
+        return int(host.size_bytes) if hasattr(host, "size_bytes") else host.numel() * host.element_size()
+
     def prefix_bytes(self, block_count: int) -> int:
         return int(block_count) * self.units_per_block * self.unit_bytes
 

@@ -127,3 +127,91 @@ def test_select_takes_many_key_heads():
     table = torch.zeros(1, 1, dtype=torch.int32).expand(2047, 1)
     with pytest.raises(ValueError, match="CUDA device"):
         ops.paged_kv_select(q, bounds, table, torch.zeros(2047, dtype=torch.int32), 1, block_size=16, recent=0)
+
+
+# ---- what leaves, as a whole: room on the host, pages that requests share ---------------------------------
+
+
+def plain_evict(mass, table, lens, budget, *, block_size, sink=1, recent=1, pages=None):
+    """What ``paged_kv_evict`` returns, on the CPU."""
+    from tests.paged_kv_cases import best
+
+    rows, width = table.shape
+    pages = 2**31 if pages is None else pages
+    kept, gone, at = (torch.full((rows, width), -1, dtype=torch.int32) for _ in range(3))
+    new_mass, new_lens, count = torch.zeros(rows, width), torch.zeros(rows, dtype=torch.int32), torch.zeros(rows, dtype=torch.int32)
+    for b in range(rows):
+        n = -(-int(lens[b]) // block_size)
+        can = [0 <= int(table[b, j]) < pages for j in range(n)]
+        stay = best(mass[b, :n].tolist(), can, budget, sink, recent)
+        out = [j for j in range(n) if can[j] and j not in stay]
+        kept[b, : len(stay)], new_mass[b, : len(stay)] = table[b, stay], mass[b, stay]
+        gone[b, : len(out)], at[b, : len(out)] = table[b, out], torch.tensor(out, dtype=torch.int32)
+        new_lens[b], count[b] = sum(min(block_size, int(lens[b]) - j * block_size) for j in stay), len(out)
+    return ops.KVEviction(kept, new_lens, new_mass, gone, at, count)
+
+
+class Recorder(PagedKVOffloader):
+    """Records its transfers instead of making them."""
+
+    def __init__(self, kvs):
+        super().__init__(Engine(), kvs, target=0, sync_stream=False)
+        self.calls = []
+
+    def save(self, block_ids, host_ptr, host_bytes, host_off=0):
+        self.calls.append((list(block_ids), host_off))
+        return len(block_ids)
+
+
+def batch():
+    table = torch.tensor([[0, 1, 2, 3, 4], [0, 1, 5, 6, -1]], dtype=torch.int32)
+    mass = torch.tensor([[9.0, 1.0, 8.0, 2.0, 0.0], [9.0, 1.0, 2.0, 0.0, 0.0]])
+    return mass, table, torch.tensor([75, 60], dtype=torch.int32)
+
+
+def test_room_for_all_that_leaves_is_checked_before_the_first_transfer(monkeypatch):
+    monkeypatch.setattr(ops, "paged_kv_evict", plain_evict)
+    store = Recorder([cache()])
+    need = store.prefix_bytes(2) + store.prefix_bytes(1)
+    for room, off in ((need - 1, 0), (need + 63, 64), (0, 0), (1 << 20, -16)):
+        with pytest.raises(ValueError, match="host region"):
+            store.evict(*batch(), 3, 4096, room, block_size=16, host_off=off)
+    assert store.calls == []
+    e, gone = store.evict(*batch(), 3, 4096, need + 64, block_size=16, host_off=64)
+    assert store.calls == [([1, 3], 64), ([1], 64 + store.prefix_bytes(2))] and len(gone) == 2
+    store.evict(*batch(), 5, 4096, 0, block_size=16)  # nothing leaves: no room is needed
+
+
+def daemon_offloader(kvs):
+    from test_daemon_landing import node
+
+    from pcie_pool_b200 import TurboBusClient
+    from pcie_pool_b200.adapters.kv_offload import DaemonKVOffloader
+
+    _, dc, sid, _ = node()
+    return DaemonKVOffloader(TurboBusClient(daemon=dc), dc, session_id=sid, job_id="job", kv_caches=kvs, units_per_chunk=4,
+                             sync_stream=False)
+
+
+def test_blocks_leave_through_the_daemon_and_come_back(monkeypatch):
+    """The mock world moves real bytes: two layers are cut, what left is saved, overwritten, and restored elsewhere."""
+    monkeypatch.setattr(ops, "paged_kv_evict", plain_evict)
+    g = torch.Generator().manual_seed(5)
+    kvs = [torch.randn(2, 16, 16, 2, 16, generator=g).to(torch.bfloat16) for _ in range(2)]
+    store = daemon_offloader(kvs)
+    mass, table, lens = batch()
+    table[1, 1], table[1, 3] = 16, 7                # an entry that is no page of the cache; no page is shared
+    table[1, 0] = 8
+    small = torch.zeros(store.prefix_bytes(3) - 1, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="host region"):
+        store.evict(mass, table, lens, 2, small, block_size=16)
+    host = torch.zeros(store.prefix_bytes(4), dtype=torch.uint8)
+    e, gone = store.evict(mass, table, lens, 2, host, block_size=16)
+    assert [(x.request, x.blocks, x.index) for x in gone] == [(0, [1, 2, 3], [1, 2, 3]), (1, [5], [2])]
+    before = [kv.clone() for kv in kvs]
+    for kv in kvs:
+        kv[:, [1, 2, 3, 5]] = 0
+    for x, pages in zip(gone, ([12, 10, 15], [11])):
+        store.restore(pages, host, host_off=x.host_off)
+        for kv, old in zip(kvs, before):
+            assert torch.equal(kv[:, pages], old[:, x.blocks])
