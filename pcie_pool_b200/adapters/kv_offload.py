@@ -13,7 +13,7 @@ request when the block table is permuted).
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Sequence
 
 import numpy as np
@@ -46,13 +46,16 @@ def kv_segments(nunits: int, host_off: int, span_blocks: int | None, nblocks: in
 @dataclass
 class EvictedKV:
     """Blocks that left a request for the host: their pages and places in the
-    request's old table, where they were saved, and the transfer."""
+    request's old table, where they were saved, the transfer, and which of the
+    pages no request of the call holds any more (each in one request's list
+    only, whoever shared it)."""
 
     request: int
     blocks: list
     index: list
     host_off: int
     stats: KVTransferStats
+    free: list = field(default_factory=list)
 
 
 class _EvictsKV:
@@ -70,8 +73,14 @@ class _EvictsKV:
         ``ops.paged_kv_attention(mass=)`` added up) and save those that leave to the host, one
         transfer for each request that loses any, one behind the other from ``host_off``; ``host``
         is what ``save`` takes.  Returns (``KVEviction``, list of ``EvictedKV``): the requests go
-        on with the eviction's table, lengths and mass, the pages of ``EvictedKV.blocks`` are free,
-        and ``restore(pages, *host, host_off=...)`` brings a request's evicted blocks back.
+        on with the eviction's table, lengths and mass, and ``restore(pages, *host, host_off=...)``
+        brings a request's evicted blocks back.
+
+        The pages of ``EvictedKV.free`` may be used for something else. Requests that share a prefix
+        are cut each by its own mass: a page that one of them keeps is not free when another loses it,
+        one that several lose is saved for each (each restores from its own region) and free once.
+        Only the rows of ``block_table`` count: a page that stands in another table too is the caller's
+        to keep.
 
         The room for all of them is checked before the first transfer (``ValueError``). The inputs
         and the cache's pages are left as they were, so after an error, of a transfer too, the caller
@@ -87,11 +96,14 @@ class _EvictsKV:
             raise ValueError(f"the {need} bytes of the blocks that leave do not fit the host region from offset {host_off} on")
         widest = max(counts, default=0)
         pages, places = e.evicted_blocks[:, :widest].tolist(), e.evicted_index[:, :widest].tolist()
+        held = set(e.block_table.unique().tolist()) if widest else set()
         out = []
         for b, n in enumerate(counts):
             if n:
                 stats = self.save(pages[b][:n], *host, host_off=host_off)
-                out.append(EvictedKV(b, pages[b][:n], places[b][:n], host_off, stats))
+                free = list(dict.fromkeys(p for p in pages[b][:n] if p not in held))
+                held.update(free)
+                out.append(EvictedKV(b, pages[b][:n], places[b][:n], host_off, stats, free))
                 host_off += self.prefix_bytes(n)
         return e, out
 

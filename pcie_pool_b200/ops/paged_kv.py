@@ -17,6 +17,7 @@ A serving step with a bounded cache strings them together::
     out = paged_kv_attention(q, kv, table, lens, mass=mass)          # every layer adds to mass
     e = paged_kv_evict(mass, table, lens, budget, block_size=16)     # pages e.evicted_blocks leave
     # PagedKVOffloader.save(...) them, then go on with e.block_table, e.context_lens, e.mass
+    # (PagedKVOffloader.evict(...) does both, and says which of the pages nobody holds any more)
 
 and one with sparse reads::
 
@@ -108,7 +109,8 @@ def paged_kv_evict(mass, block_table, context_lens, budget, *, block_size, sink=
     stays the last.  Blocks that are not resident take no place in the
     budget, are dropped and not listed: negative table entries, and with ``pages``,
     the cache's number of pages, entries from there on too (without it every other
-    entry is taken for a page).  The inputs are left as they were.
+    entry is taken for a page).  Requests are cut each on its own: a page that two of
+    them share may leave one and stay with the other.  The inputs are left as they were.
     """
     return KVEviction(*native_kv().evict(mass, block_table, context_lens, budget, block_size, sink, recent,
                                           pages))

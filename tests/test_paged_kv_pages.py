@@ -215,3 +215,17 @@ def test_blocks_leave_through_the_daemon_and_come_back(monkeypatch):
         store.restore(pages, host, host_off=x.host_off)
         for kv, old in zip(kvs, before):
             assert torch.equal(kv[:, pages], old[:, x.blocks])
+
+
+def test_pages_that_requests_share_are_free_once_nobody_keeps_them(monkeypatch):
+    monkeypatch.setattr(ops, "paged_kv_evict", plain_evict)
+    # page 1: both lose it; page 2: the first keeps it, the second loses it; page 4 stands twice in one row and leaves twice
+    table = torch.tensor([[0, 1, 2, 3, 9], [0, 1, 2, 6, 9], [4, 5, 4, 7, 8]], dtype=torch.int32)
+    mass = torch.tensor([[9.0, 1.0, 8.0, 2.0, 0.0], [9.0, 1.0, 2.0, 5.0, 0.0], [1.0, 9.0, 1.0, 8.0, 0.0]])
+    store = Recorder([torch.zeros(2, 16, 16, 2, 64, dtype=torch.bfloat16)])
+    e, gone = store.evict(mass, table, torch.tensor([80, 80, 80], dtype=torch.int32), 3, 4096, 1 << 20, block_size=16, sink=0)
+    assert e.block_table[:, :3].tolist() == [[0, 2, 9], [0, 6, 9], [5, 7, 8]]
+    assert [(x.blocks, x.free) for x in gone] == [([1, 3], [1, 3]), ([1, 2], []), ([4, 4], [4])]
+    # every request has all its blocks on the host, in a region of its own
+    assert [c[0] for c in store.calls] == [[1, 3], [1, 2], [4, 4]]
+    assert [c[1] for c in store.calls] == [0, store.prefix_bytes(2), store.prefix_bytes(4)]
