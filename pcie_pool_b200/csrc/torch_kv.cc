@@ -150,7 +150,7 @@ py::object kv_attention(const Tensor& given, const Tensor& kv, const Tensor& tab
          "out must be contiguous, like q, on a 4-byte boundary");
     need(!overlaps(*out, q) && !overlaps(*out, kv), "out must not overlap q or kv");
   }
-  const cudaStream_t stream = stream_of({&kv, &q});
+  const cudaStream_t stream = stream_of({&kv, &q, mass ? &*mass : &kv, out ? &*out : &kv});
   if (!out) out = empty(q.sizes(), q.scalar_type(), device);
   const Tensor lse = empty({n, a.q.heads}, at::kFloat, device);
   if (blocks && a.blocks_width == 0) {

@@ -229,3 +229,25 @@ def test_pages_that_requests_share_are_free_once_nobody_keeps_them(monkeypatch):
     # every request has all its blocks on the host, in a region of its own
     assert [c[0] for c in store.calls] == [[1, 3], [1, 2], [4, 4]]
     assert [c[1] for c in store.calls] == [0, store.prefix_bytes(2), store.prefix_bytes(4)]
+
+
+# ---- what the operators write to -------------------------------------------------------------------------
+
+
+@pytest.fixture
+def good():
+    from tests.paged_kv_cases import make
+
+    q, kv, table, lens = make(0, [20, 5], 16, 8, 2, 64, torch.bfloat16)
+    return dict(q=q, kv=kv, block_table=table, context_lens=lens)
+
+
+@pytest.mark.parametrize("name", ["mass", "out", "kv", "q"])
+def test_attention_refuses_what_requires_a_gradient(good, name):
+    """mass and out are written in place: autograd would not see it."""
+    given = dict(good, mass=torch.zeros(good["block_table"].shape), out=torch.empty_like(good["q"]))
+    given[name] = given[name].clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.paged_kv_attention(**given)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+        ops.paged_kv_attention(**given)
