@@ -107,13 +107,22 @@ Tensor query_of(const Tensor& given, const at::Device& device, at::ScalarType ty
   return q;
 }
 
-// Whether a contiguous tensor shares memory with what another spans.
-bool overlaps(const Tensor& t, const Tensor& other) {
-  if (t.numel() == 0 || other.numel() == 0) return false;
+uintptr_t end_of(const Tensor& t) {
   int64_t last = 0;
-  for (int64_t i = 0; i < other.dim(); ++i) last += (other.size(i) - 1) * other.stride(i);
-  const uintptr_t end = address(other) + (last + 1) * other.element_size();
-  return address(t) < end && address(other) < address(t) + t.numel() * t.element_size();
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return address(t) + (last + 1) * t.element_size();
+}
+
+// Whether what two tensors span has memory in common.  Rows of one buffer that stand
+// next to each other (equal strides) do not.
+bool overlaps(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  if (address(a) >= end_of(b) || address(b) >= end_of(a)) return false;
+  if (a.dim() != 2 || b.dim() != 2 || a.size(0) < 2 || b.size(0) < 2) return true;
+  const uintptr_t pitch = a.stride(0) * a.element_size(), row_a = a.size(1) * a.element_size(), row_b = b.size(1) * b.element_size();
+  if (pitch != b.stride(0) * b.element_size() || row_a > pitch || row_b > pitch) return true;
+  const uintptr_t apart = address(b) >= address(a) ? (address(b) - address(a)) % pitch : (pitch - (address(a) - address(b)) % pitch) % pitch;
+  return apart < row_a || apart + row_b > pitch;
 }
 
 py::object kv_attention(const Tensor& given, const Tensor& kv, const Tensor& table, const Tensor& lens,
@@ -141,6 +150,8 @@ py::object kv_attention(const Tensor& given, const Tensor& kv, const Tensor& tab
          "mass must be fp32 in block_table's shape");
     need((width <= 1 || mass->stride(1) == 1) && (n <= 1 || mass->stride(0) >= width),
          "mass must have contiguous rows of their own");
+    need(!overlaps(*mass, q) && !overlaps(*mass, kv) && !overlaps(*mass, table) && !overlaps(*mass, lens),
+         "mass must not overlap q, kv, block_table or context_lens");
     a.mass = mass->data_ptr<float>();
     a.mass_stride = mass->stride(0);
   }
@@ -148,7 +159,9 @@ py::object kv_attention(const Tensor& given, const Tensor& kv, const Tensor& tab
     need(out->scalar_type() == q.scalar_type() && out->device() == device && out->sizes() == q.sizes() &&
              out->is_contiguous() && address(*out) % 4 == 0,
          "out must be contiguous, like q, on a 4-byte boundary");
-    need(!overlaps(*out, q) && !overlaps(*out, kv), "out must not overlap q or kv");
+    need(!overlaps(*out, q) && !overlaps(*out, kv) && !overlaps(*out, table) && !overlaps(*out, lens) &&
+             !(blocks && overlaps(*out, *blocks)) && !(mass && overlaps(*out, *mass)),
+         "out must not overlap q, kv or another argument");
   }
   const cudaStream_t stream = stream_of({&kv, &q, mass ? &*mass : &kv, out ? &*out : &kv});
   if (!out) out = empty(q.sizes(), q.scalar_type(), device);
@@ -175,7 +188,8 @@ void kv_bounds(const Tensor& kv, const Tensor& table, const Tensor& lens, const 
            bounds.size(0) == cache.pages && bounds.size(1) == cache.kv_heads && bounds.size(2) == 2 &&
            bounds.size(3) == cache.dim && bounds.is_contiguous() && address(bounds) % 16 == 0,
        "bounds must be contiguous [pages, kv_heads, 2, dim] in the cache's type, on a 16-byte boundary");
-  need(!overlaps(bounds, kv), "bounds must not overlap kv");
+  need(!overlaps(bounds, kv) && !overlaps(bounds, table) && !overlaps(bounds, lens),
+       "bounds must not overlap kv, block_table or context_lens");
   const int since = !new_tokens.is_none() ? whole(new_tokens, 0, "new_tokens must be an integer >= 0") : -1;
   const cudaStream_t stream = stream_of({&kv, &bounds});
   DeviceGuard guard(kv.get_device());

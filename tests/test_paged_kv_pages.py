@@ -251,3 +251,50 @@ def test_attention_refuses_what_requires_a_gradient(good, name):
         ops.paged_kv_attention(**given)
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
         ops.paged_kv_attention(**given)
+
+
+def shared(dtype, shape, with_shape, with_dtype, at=0):
+    """Two tensors in one buffer: the second begins `at` bytes behind the first."""
+    buf = torch.zeros(1 << 16, dtype=torch.uint8)
+    one, two = (torch.empty(s, dtype=t) for s, t in ((shape, dtype), (with_shape, with_dtype)))
+    size = [x.numel() * x.element_size() for x in (one, two)]
+    return (buf[: size[0]].view(dtype).view(shape), buf[at: at + size[1]].view(with_dtype).view(with_shape))
+
+
+@pytest.mark.parametrize("written,read", [("out", "block_table"), ("out", "context_lens"), ("out", "blocks"), ("out", "mass"),
+                                          ("mass", "q"), ("mass", "kv"), ("mass", "block_table"), ("mass", "context_lens"),
+                                          ("bounds", "block_table"), ("bounds", "context_lens")])
+def test_what_is_written_must_not_share_memory_with_what_is_read(good, written, read):
+    kv = good["kv"][:, :3].contiguous()
+    args = dict(good, kv=kv, blocks=torch.zeros(2, 2, 1, dtype=torch.int32), mass=torch.zeros(good["block_table"].shape),
+                out=torch.empty_like(good["q"]), bounds=torch.zeros(3, 2, 2, 64, dtype=kv.dtype))
+    args.pop("mass" if "blocks" in (written, read) else "blocks")  # they do not go together
+    w, r = args[written], args[read]
+    args[written], args[read] = shared(w.dtype, w.shape, r.shape, r.dtype)
+    if written == "bounds":
+        with pytest.raises(ValueError, match="must not overlap"):
+            ops.paged_kv_bounds(args["kv"], args["block_table"], args["context_lens"], args["bounds"])
+        return
+    args.pop("bounds")
+    with pytest.raises(ValueError, match="must not overlap"):
+        ops.paged_kv_attention(**args)
+
+
+def test_neighbours_in_one_buffer_do_not_overlap(good):
+    width = good["block_table"].shape[1]
+    rows = torch.zeros(2, 4 * width, dtype=torch.int32)   # table and mass side by side, in both orders, and behind each other
+    for first, second in ((0, 1), (1, 0), (3, 2), (0, 3)):
+        table = rows[:, first * width: (first + 1) * width].copy_(good["block_table"])
+        mass = rows.view(torch.float32)[:, second * width: (second + 1) * width]
+        with pytest.raises(ValueError, match="CUDA device"):
+            ops.paged_kv_attention(**dict(good, block_table=table), mass=mass)
+    for off in (1, width - 1):                            # a column in common
+        with pytest.raises(ValueError, match="must not overlap"):
+            ops.paged_kv_attention(**dict(good, block_table=rows[:, width: 2 * width]),
+                                   mass=rows.view(torch.float32)[:, width + off: 2 * width + off])
+        with pytest.raises(ValueError, match="must not overlap"):
+            ops.paged_kv_attention(**dict(good, block_table=rows[:, width: 2 * width]),
+                                   mass=rows.view(torch.float32)[:, width - off: 2 * width - off])
+    out, mass = shared(good["q"].dtype, good["q"].shape, (2, width), torch.float32, at=good["q"].numel() * 2)
+    with pytest.raises(ValueError, match="CUDA device"):
+        ops.paged_kv_attention(**good, out=out, mass=mass)
