@@ -107,6 +107,11 @@ Tensor query_of(const Tensor& given, const at::Device& device, at::ScalarType ty
   return q;
 }
 
+// Tells autograd that a tensor of the caller's is written: a graph that saved it then says so in its backward pass.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 uintptr_t end_of(const Tensor& t) {
   int64_t last = 0;
   for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
@@ -164,6 +169,8 @@ py::object kv_attention(const Tensor& given, const Tensor& kv, const Tensor& tab
          "out must not overlap q, kv or another argument");
   }
   const cudaStream_t stream = stream_of({&kv, &q, mass ? &*mass : &kv, out ? &*out : &kv});
+  if (out) written(*out);
+  if (mass) written(*mass);
   if (!out) out = empty(q.sizes(), q.scalar_type(), device);
   const Tensor lse = empty({n, a.q.heads}, at::kFloat, device);
   if (blocks && a.blocks_width == 0) {
@@ -192,6 +199,7 @@ void kv_bounds(const Tensor& kv, const Tensor& table, const Tensor& lens, const 
        "bounds must not overlap kv, block_table or context_lens");
   const int since = !new_tokens.is_none() ? whole(new_tokens, 0, "new_tokens must be an integer >= 0") : -1;
   const cudaStream_t stream = stream_of({&kv, &bounds});
+  written(bounds);
   DeviceGuard guard(kv.get_device());
   check_cuda(paged_kv_bounds(cache, req, since, bounds.data_ptr(), stream), "paged_kv_bounds");
 }

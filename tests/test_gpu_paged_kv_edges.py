@@ -129,3 +129,25 @@ def test_large_values_in_fp16(need_gpu, heads, kv_heads):
     kv[1][..., 0] = kv[1][..., 0].abs()
     out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), scale=0.25, return_lse=True)
     check_attention(q, kv, table, lens, out, lse, scale=0.25)
+
+
+# ---- what is written, and autograd -------------------------------------------------------------------------
+
+
+def test_what_is_written_is_known_to_autograd(need_gpu):
+    q, kv, table, lens = (t.cuda() for t in make(74, [40, 5], 16, 8, 2, 64, BF16))
+    w = torch.ones(q.shape, dtype=BF16, device="cuda", requires_grad=True)
+    m = torch.ones(table.shape, device="cuda", requires_grad=True)
+    b = torch.ones(kv.shape[1], 2, 2, 64, dtype=BF16, device="cuda", requires_grad=True)
+    out, mass, bounds = torch.zeros_like(q), torch.zeros(table.shape, device="cuda"), torch.zeros_like(b, requires_grad=False)
+    graphs = [(w * out).sum(), (m * mass).sum(), (b * bounds).sum()]  # each saves what is written below
+    ops.paged_kv_attention(q, kv, table, lens, out=out, mass=mass)
+    ops.paged_kv_bounds(kv, table, lens, bounds)
+    assert out._version == 1 and mass._version == 1 and bounds._version == 1
+    for loss in graphs:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():  # tensors that have no versions
+        out = torch.zeros_like(q)
+        ops.paged_kv_attention(q, kv, table, lens, out=out)
+        assert out.abs().sum() > 0
