@@ -83,8 +83,9 @@ PagedKv cache_of(const Tensor& kv) {
        "kv's dim must be a multiple of 8 from 8 to 256, and it must have heads and tokens");
   need(kv.size(1) < kInt && kv.size(2) < kInt && kv.size(3) < kInt / kMaxDim, "too many pages, tokens of a page or heads");
   need(kv.stride(4) == 1, "kv's last dimension must be contiguous");
-  need(address(kv) % 16 == 0 && (kv.stride(0) | kv.stride(1) | kv.stride(2) | kv.stride(3)) % 8 == 0,
-       "kv's address and strides must be multiples of 16 bytes");
+  int64_t strides = 0;  // of a dimension of one nothing is multiplied
+  for (int i = 0; i < 4; ++i) strides |= kv.size(i) > 1 ? kv.stride(i) : 0;
+  need(address(kv) % 16 == 0 && strides % 8 == 0, "kv's address and strides must be multiples of 16 bytes");
   return {kv.data_ptr(), kv.stride(0), kv.stride(1), kv.stride(2), kv.stride(3), static_cast<int>(kv.size(1)),
           static_cast<int>(kv.size(2)), static_cast<int>(kv.size(3)), static_cast<int>(dim), type};
 }

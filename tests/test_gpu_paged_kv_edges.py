@@ -151,3 +151,21 @@ def test_what_is_written_is_known_to_autograd(need_gpu):
         out = torch.zeros_like(q)
         ops.paged_kv_attention(q, kv, table, lens, out=out)
         assert out.abs().sum() > 0
+
+
+# ---- layouts ---------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim,lens,block,kv_heads", [(1, [9], 16, 2), (2, [3, 4], 1, 2), (3, [70, 5], 16, 1)])
+def test_any_stride_of_a_dimension_of_one(need_gpu, dim, lens, block, kv_heads):
+    q, kv, table, lens = make(75, lens, block, 2 * kv_heads, kv_heads, 64, BF16, pages_extra=0)
+    assert kv.shape[dim] == 1
+    strides = list(kv.stride())
+    strides[dim] = 3
+    odd = kv.cuda().as_strided(kv.shape, strides)
+    out, lse = ops.paged_kv_attention(q.cuda(), odd, table.cuda(), lens.cuda(), return_lse=True)
+    check_attention(q, kv, table, lens, out, lse)
+    bounds = [torch.zeros(kv.shape[1], kv_heads, 2, 64, dtype=BF16, device="cuda") for _ in range(2)]
+    for k, b in zip((odd, kv.cuda()), bounds):
+        ops.paged_kv_bounds(k, table.cuda(), lens.cuda(), b)
+    assert torch.equal(*bounds)

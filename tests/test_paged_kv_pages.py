@@ -298,3 +298,18 @@ def test_neighbours_in_one_buffer_do_not_overlap(good):
     out, mass = shared(good["q"].dtype, good["q"].shape, (2, width), torch.float32, at=good["q"].numel() * 2)
     with pytest.raises(ValueError, match="CUDA device"):
         ops.paged_kv_attention(**good, out=out, mass=mass)
+
+
+def test_strides_of_dimensions_of_one_do_not_count():
+    """A cache of one page, one head or one token a page: torch gives such a dimension any stride."""
+    flat = torch.zeros(1 << 14, dtype=torch.bfloat16)
+    q, table, lens = torch.zeros(1, 4, 64, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    sizes, strides = [2, 4, 16, 2, 64], [4096, 1024, 64, 2048, 1]
+    for i in (1, 2, 3):
+        one = [1 if j == i else n for j, n in enumerate(sizes)]
+        odd = [3 if j == i else n for j, n in enumerate(strides)]
+        kv = flat.as_strided(one, odd)
+        with pytest.raises(ValueError, match="CUDA device"):
+            ops.paged_kv_attention(q, kv, table, lens)
+        with pytest.raises(ValueError, match="multiples of 16 bytes"):
+            ops.paged_kv_attention(q, flat.as_strided(sizes, odd), table, lens)
