@@ -127,8 +127,9 @@ __global__ void __launch_bounds__(256, 2)
 // the bits of a bf16 or fp16 value, moved to where a double keeps its exponent and
 // mantissa, are that value times a power of two, subnormals and zero included.
 // A and B carry half of that power, and the sum gets the other half back.  Infinities
-// and values that are not a number do not move so; a row that has one (0 * x tells)
-// is summed again with converted values.
+// and values that are not a number do not move so; where a row has one (0 * x tells)
+// the eight are summed again with converted values, in the same order, so that a
+// block's score does not hang on its neighbours.
 constexpr int kScoreWarps = 8, kTogether = 8, kReach = 128;
 
 template <typename T>
@@ -292,8 +293,14 @@ __global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_co
             uint2 top, low;
             bounds_of(i, p, top, low);
             const float2 a0 = floats<T>(top.x), a1 = floats<T>(top.y), b0 = floats<T>(low.x), b1 = floats<T>(low.y);
-            sum[i] += above[p][0] * a0.x + above[p][1] * a0.y + above[p][2] * a1.x + above[p][3] * a1.y;
-            sum[i] += below[p][0] * b0.x + below[p][1] * b0.y + below[p][2] * b1.x + below[p][3] * b1.y;
+            sum[i] += above[p][0] * a0.x;
+            sum[i] += above[p][1] * a0.y;
+            sum[i] += above[p][2] * a1.x;
+            sum[i] += above[p][3] * a1.y;
+            sum[i] += below[p][0] * b0.x;
+            sum[i] += below[p][1] * b0.y;
+            sum[i] += below[p][2] * b1.x;
+            sum[i] += below[p][3] * b1.y;
           }
         }
       }

@@ -169,3 +169,24 @@ def test_any_stride_of_a_dimension_of_one(need_gpu, dim, lens, block, kv_heads):
     for k, b in zip((odd, kv.cuda()), bounds):
         ops.paged_kv_bounds(k, table.cuda(), lens.cuda(), b)
     assert torch.equal(*bounds)
+
+
+# ---- scores -----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("other", ["nothing", "nan", "inf"])
+@pytest.mark.parametrize("dim", [8, 256])
+def test_a_score_does_not_hang_on_its_neighbours(need_gpu, other, dim):
+    """Block 1 is 1 + 2^-24 and two numbers that 64 bits round away one by one, but not when they are added first: it would
+    then round to more than the 1 of block 0.  A neighbour that is not finite must not change how it is summed."""
+    bounds = torch.zeros(9, 1, 2, dim, dtype=BF16)
+    bounds[0, 0, 1, 0] = 1.0
+    bounds[1, 0, 1, :2] = torch.tensor([1.0, 2.0 ** -24])
+    bounds[1, 0, 0, 2:4] = -3 * 2.0 ** -55
+    if other != "nothing":
+        bounds[2, 0, :, 0] = -math.inf if other == "inf" else math.nan
+    q = torch.zeros(1, 1, dim, dtype=BF16)
+    q[0, 0, :4] = torch.tensor([1.0, 1.0, -1.0, -1.0])
+    table, lens = torch.arange(9, dtype=torch.int32)[None].cuda(), torch.tensor([9], dtype=torch.int32).cuda()
+    got = ops.paged_kv_select(q.cuda(), bounds.cuda(), table, lens, 1, block_size=1, sink=0, recent=0)
+    assert got.tolist() == [[[0]]]
