@@ -57,6 +57,12 @@ def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=N
     attention weight that the heads gave to each block, summed over heads and
     tokens, so a request's row grows by ``heads`` in all.  It needs a block size
     that is a multiple of 16 and at most 1024 heads, and takes no ``blocks``.
+
+    What is not finite in a token that counts shows, and nowhere else: a value that
+    is infinite or no number makes that channel of its heads' results infinite or no
+    number; a score of minus infinity counts for nothing; one of plus infinity or no
+    number makes the head's result, its log-sum and the mass of its request no number.
+    Other places of the cache may hold anything.
     """
     return native_kv().attention(q, kv, block_table, context_lens, scale, blocks, mass, out, return_lse)
 
@@ -80,7 +86,8 @@ def paged_kv_select(q, bounds, block_table, context_lens, keep, *, block_size, s
     A block's score is the largest that ``q . k`` could be for a key within the
     block's ``bounds`` (``paged_kv_bounds``), summed over the group's heads:
     ``sum_h sum_d max(q_hd * lo_d, q_hd * hi_d)``, summed in 64 bits and rounded to
-    fp32 once.  The first ``sink`` and the last ``recent`` blocks are always
+    fp32 once.  A channel whose query is 0 adds nothing whatever its bounds are, and of
+    two bounds the one that is a number counts.  The first ``sink`` and the last ``recent`` blocks are always
     taken, the others by score, ties to the lowest index; a score that is not a
     number ranks lowest.  ``bounds`` may have more rows than the cache has pages:
     a table of its own then also ranks blocks that are offloaded.  Entries that

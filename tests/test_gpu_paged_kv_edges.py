@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from pcie_pool_b200 import ops  # noqa: E402
-from tests.paged_kv_cases import best, make, to_gpu  # noqa: E402
+from tests.paged_kv_cases import attention, best, make  # noqa: E402
 
 BF16, FP16 = torch.bfloat16, torch.float16
 
@@ -190,3 +190,54 @@ def test_a_score_does_not_hang_on_its_neighbours(need_gpu, other, dim):
     table, lens = torch.arange(9, dtype=torch.int32)[None].cuda(), torch.tensor([9], dtype=torch.int32).cuda()
     got = ops.paged_kv_select(q.cuda(), bounds.cuda(), table, lens, 1, block_size=1, sink=0, recent=0)
     assert got.tolist() == [[[0]]]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_channel_without_a_query_adds_nothing_to_a_score(need_gpu, dtype):
+    bounds = torch.zeros(5, 1, 2, 8, dtype=dtype)
+    bounds[0, 0, 1, 0] = 1.0
+    bounds[1, 0, 1, 0], bounds[1, 0, 1, 3], bounds[1, 0, 0, 4] = 2.0, math.inf, math.nan   # channels 3 and 4 have no query
+    bounds[2, 0, 0, 0], bounds[2, 0, 1, 0] = math.nan, 3.0
+    bounds[3, 0, 0, 0], bounds[3, 0, 1, 0] = 4.0, math.nan
+    bounds[4, 0, :, 0] = math.nan
+    q = torch.zeros(1, 2, 8, dtype=dtype)
+    q[0, :, 0] = torch.tensor([1.0, 0.0])
+    table, lens = torch.arange(5, dtype=torch.int32)[None].cuda(), torch.tensor([5], dtype=torch.int32).cuda()
+    for keep, want in enumerate(([3], [2, 3], [1, 2, 3], [0, 1, 2, 3], [0, 1, 2, 3, 4]), 1):
+        got = ops.paged_kv_select(q.cuda(), bounds.cuda(), table, lens, keep, block_size=1, sink=0, recent=0)
+        assert got[0, 0].tolist() == want
+
+
+# ---- what is not finite --------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("heads", [4, 24])
+@pytest.mark.parametrize("tokens", [40, 3000])
+def test_what_is_not_finite_shows_where_it_counts(need_gpu, dtype, heads, tokens):
+    q, kv, table, lens = make(76, [tokens] * 4, 16, heads, 2, 64, dtype)
+    G = heads // 2
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    kv[1, table[0, 1], 3, 1, 5] = math.inf       # a value: channel 5 of the second key head's queries
+    kv[1, table[1, 1], 3, 0, 6] = -math.inf
+    kv[0, table[2, 0], 7, 1, 0] = math.inf       # a key: scores of plus infinity
+    kv[0, table[3, 0], 7, 0, 0] = -math.inf      # of minus infinity, whose value does not matter
+    kv[1, table[3, 0], 7, 0] = 0.0
+    mass = torch.zeros(table.shape, device="cuda")
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), mass=mass, return_lse=True)
+    bad = ~torch.isfinite(out).cpu()
+    want = torch.zeros_like(bad)
+    want[0, G:, 5] = want[1, :G, 6] = want[2, G:] = True
+    assert torch.equal(bad, want)
+    assert torch.isnan(out[2, G:]).all() and torch.isnan(lse[2, G:]).all()
+    assert torch.isfinite(lse[:2]).all() and torch.isfinite(lse[2, :G]).all() and torch.isfinite(lse[3]).all()
+    n = -(-tokens // 16)
+    assert torch.isfinite(mass[[0, 1, 3]]).all() and torch.isnan(mass[2, :n]).all() and (mass[2, n:] == 0).all()
+    # the first key head's token of minus infinity as if it were not there: the last one in its place
+    page, at = table[3, (tokens - 1) // 16], (tokens - 1) % 16
+    without = kv.clone()
+    without[:, table[3, 0], 7, 0] = kv[:, page, at, 0]
+    for rows, cache, length in ((slice(0, G), without, tokens - 1), (slice(G, heads), kv, tokens)):
+        ref, _, _, err, _ = attention(q[3:], cache, table[3:], torch.tensor([length]))
+        tol = err + torch.finfo(dtype).eps / 2 * (ref.abs() + err) + (2.0 ** -25 if dtype == FP16 else 0.0)
+        assert ((out[3:].cpu().double() - ref).abs() <= tol)[:, rows].all()
