@@ -40,12 +40,15 @@ def extension_path(name: str = "_C") -> Path:
     return PKG_DIR / f"{name}{suffix}"
 
 
-def _torch_paths() -> tuple[str, Path]:
-    """torch's version and folder, without importing it."""
+def _torch_paths() -> tuple[str, Path] | None:
+    """torch's version and folder, without importing it; None where it is not installed."""
     import importlib.metadata
     import importlib.util
 
-    return importlib.metadata.version("torch"), Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    return importlib.metadata.version("torch"), Path(spec.submodule_search_locations[0])
 
 
 def _includes() -> list[str]:
@@ -80,17 +83,17 @@ def _compile(cmd: list[str]) -> None:
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile (if needed) and link ``_C`` and ``_kv``; returns ``_C``'s path."""
+    """Compile (if needed) and link ``_C``, then ``_kv``; returns ``_C``'s path.
+    ``_C`` needs neither torch nor that ``_kv`` can be built; without torch ``_kv``
+    is left out."""
     BUILD_DIR.mkdir(exist_ok=True)
     nvcc = str(CUDA_HOME / "bin" / "nvcc")
     inc = _includes()
     head = _newest_header()
-    version, torch_dir = _torch_paths()
-    torch_inc = [f"-I{CSRC}", f"-isystem{torch_dir / 'include'}", f"-isystem{torch_dir / 'include/torch/csrc/api/include'}",
-                 f"-I{sysconfig.get_paths()['include']}", f"-I{CUDA_HOME / 'include'}"]
-    cmds: list[list[str]] = []
+    torch_paths = _torch_paths()
 
-    def objects(names: list[str], compiler: list[str], includes: list[str], tag: str = "") -> list[Path]:
+    def objects(cmds: list, names: list[str], compiler: list[str], includes: list[str], tag: str = "") -> list[Path]:
+        """Objects of the sources; what has to be compiled for them joins ``cmds``."""
         objs = []
         for name in names:
             src, obj = CSRC / name, BUILD_DIR / f"{name}{tag}.o"
@@ -101,21 +104,31 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
 
     cuda = [nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
     host = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden"]
-    core = objects(CU_SOURCES, cuda, inc) + objects(CC_SOURCES, host, inc)
-    core_changed = bool(cmds)
-    kv = objects(KV_CU_SOURCES, cuda, [f"-I{CSRC}"])
-    # its objects are one torch version's
-    kv += objects(KV_CC_SOURCES, [*host, "-DTORCH_EXTENSION_NAME=_kv"], torch_inc, f".torch-{version}")
-    kv_changed = any(str(o) in c for c in cmds for o in kv)
-    if cmds:
-        with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 4)) as pool:
-            list(pool.map(_compile, cmds))
     cudart = [f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static", "-lrt", "-lpthread", "-ldl"]
-    out = extension_path()
-    if force or core_changed or not out.exists():
-        _compile(["g++", "-shared", "-o", str(out), *map(str, core), *cudart])
+    core_cmds: list[list[str]] = []
+    kv_cmds: list[list[str]] = []
+    core = objects(core_cmds, CU_SOURCES, cuda, inc) + objects(core_cmds, CC_SOURCES, host, inc)
+    if torch_paths:
+        version, torch_dir = torch_paths
+        torch_inc = [f"-I{CSRC}", f"-isystem{torch_dir / 'include'}", f"-isystem{torch_dir / 'include/torch/csrc/api/include'}",
+                     f"-I{sysconfig.get_paths()['include']}", f"-I{CUDA_HOME / 'include'}"]
+        kv = objects(kv_cmds, KV_CU_SOURCES, cuda, [f"-I{CSRC}"])
+        # its objects are one torch version's
+        kv += objects(kv_cmds, KV_CC_SOURCES, [*host, "-DTORCH_EXTENSION_NAME=_kv"], torch_inc, f".torch-{version}")
+    with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 4)) as pool:
+        core_runs, kv_runs = ([pool.submit(_compile, c) for c in cmds] for cmds in (core_cmds, kv_cmds))
+        for run in core_runs:
+            run.result()
+        out = extension_path()
+        if force or core_cmds or not out.exists():
+            _compile(["g++", "-shared", "-o", str(out), *map(str, core), *cudart])
+        for run in kv_runs:
+            run.result()
+    if not torch_paths:
+        print(f"built {out}; torch is not installed, so the paged-KV operators (_kv) are left out")
+        return out
     kv_out, stamp = extension_path("_kv"), BUILD_DIR / "_kv.torch"
-    if force or kv_changed or not kv_out.exists() or not stamp.exists() or stamp.read_text() != version:
+    if force or kv_cmds or not kv_out.exists() or not stamp.exists() or stamp.read_text() != version:
         # torch is imported before the module: its libraries are found by their names
         _compile(["g++", "-shared", "-o", str(kv_out), *map(str, kv), f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda",
                   "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,--exclude-libs,ALL", *cudart])
