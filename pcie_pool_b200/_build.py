@@ -114,7 +114,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
                      f"-I{sysconfig.get_paths()['include']}", f"-I{CUDA_HOME / 'include'}"]
         kv = objects(kv_cmds, KV_CU_SOURCES, cuda, [f"-I{CSRC}"])
         # its objects are one torch version's
-        kv += objects(kv_cmds, KV_CC_SOURCES, [*host, "-DTORCH_EXTENSION_NAME=_kv"], torch_inc, f".torch-{version}")
+        kv += objects(kv_cmds, KV_CC_SOURCES, [*host, "-DTORCH_EXTENSION_NAME=_kv", f'-DPPB_TORCH="{version}"'], torch_inc, f".torch-{version}")
     with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 4)) as pool:
         core_runs, kv_runs = ([pool.submit(_compile, c) for c in cmds] for cmds in (core_cmds, kv_cmds))
         for run in core_runs:

@@ -34,7 +34,10 @@ def native_kv() -> ModuleType:
     building it in-tree if needed."""
     global _KV
     if _KV is None:
-        import torch  # noqa: F401  (its libraries are the module's)
+        try:
+            import torch  # noqa: F401  (its libraries are the module's)
+        except ImportError as exc:
+            raise RuntimeError("the paged-KV operators need torch") from exc
 
         _KV = _load("pcie_pool_b200._kv", True)
     return _KV
@@ -55,6 +58,7 @@ def _load(name: str, build_if_missing: bool) -> ModuleType:
         "pcie_pool_b200 native extension is not built; run "
         "`python -m pcie_pool_b200._build`"
         + (" (a GPU is visible, so no fallback is used)" if _gpu_visible() else "")
+        + f": {_ERR}"
     ) from _ERR
 
 

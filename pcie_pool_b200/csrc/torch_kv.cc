@@ -275,6 +275,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> kv_evict(const Tensor
 }  // namespace
 
 PYBIND11_MODULE(_kv, m) {
+  // torch's C++ classes are laid out by version: a module of another one must not run
+  const auto version = py::str(py::module_::import("torch").attr("__version__")).cast<std::string>();
+  if (version != PPB_TORCH)
+    throw py::import_error("pcie_pool_b200._kv was built for torch " PPB_TORCH ", this is torch " + version +
+                           ": run `python -m pcie_pool_b200._build` and start anew");
   m.doc() = "paged-KV operators on torch tensors (sm_100a kernels)";
   m.def("attention", &kv_attention);
   m.def("bounds", &kv_bounds);

@@ -50,3 +50,22 @@ def test_the_core_is_linked_before_the_operators_fail(commands, monkeypatch):
     with pytest.raises(RuntimeError, match="native build failed"):
         _build.build()
     assert made(commands)[1] == ["_C.so"]
+
+
+def run(code):
+    import os
+    import subprocess
+    import sys
+
+    return subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=Path(__file__).resolve().parents[1], env={**os.environ, "PCIE_POOL_NO_BUILD": "1"})
+
+
+def test_a_module_of_another_torch_version_is_not_loaded():
+    r = run("import torch\ntorch.__version__ = '1.0'\nfrom pcie_pool_b200._native import native_kv\nnative_kv()")
+    assert r.returncode != 0 and "was built for torch" in r.stderr and "this is torch 1.0" in r.stderr
+
+
+def test_the_operators_name_what_they_need_where_torch_is_missing():
+    r = run("import sys\nsys.modules['torch'] = None\nfrom pcie_pool_b200._native import native, native_kv\nnative()\nnative_kv()")
+    assert r.returncode != 0 and "RuntimeError: the paged-KV operators need torch" in r.stderr
