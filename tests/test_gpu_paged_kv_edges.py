@@ -241,3 +241,60 @@ def test_what_is_not_finite_shows_where_it_counts(need_gpu, dtype, heads, tokens
         ref, _, _, err, _ = attention(q[3:], cache, table[3:], torch.tensor([length]))
         tol = err + torch.finfo(dtype).eps / 2 * (ref.abs() + err) + (2.0 ** -25 if dtype == FP16 else 0.0)
         assert ((out[3:].cpu().double() - ref).abs() <= tol)[:, rows].all()
+
+
+# ---- the largest numbers of requests and tokens a page ------------------------------------------------------------
+
+
+def test_mass_of_more_requests_than_ranges(need_gpu):
+    lens = [(i * 37) % 90 for i in range(700)]
+    q, kv, table, lens = make(77, lens, 16, 4, 2, 64, FP16)
+    mass = torch.zeros(table.shape, device="cuda")
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), mass=mass, return_lse=True)
+    weight, lse_err = check_attention(q, kv, table, lens, out, lse)
+    tol = weight * (3 * lse_err.amax(1, keepdim=True) + 84 * 2.0 ** -24 + 2.0 ** -20) + 2.0 ** -24 * weight
+    assert ((mass.cpu().double() - weight).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16), (256, BF16)])
+def test_the_most_requests(need_gpu, dim, dtype):
+    """4096 requests of 0 to 6 tokens, two of them long: attention, bounds, selection and eviction."""
+    from tests.paged_kv_cases import scores
+
+    lens = [i % 7 for i in range(4096)]
+    lens[1000], lens[4095] = 500, 333
+    q, kv, table, lens = make(78, lens, 16, 2, 1, dim, dtype)
+    qg, kg, tg, lg = (t.cuda() for t in (q, kv, table, lens))
+    mass = torch.zeros(table.shape, device="cuda")
+    out, lse = ops.paged_kv_attention(qg, kg, tg, lg, mass=mass, return_lse=True)
+    weight, _ = check_attention(q, kv, table, lens, out, lse)
+    assert ((mass.cpu().double() - weight).abs() <= 1e-4 * weight + 1e-6).all()
+    bounds = torch.zeros(kv.shape[1], 1, 2, dim, dtype=dtype)
+    for b in range(4096):
+        for j in range(-(-int(lens[b]) // 16)):
+            k = kv[0, table[b, j], : min(16, int(lens[b]) - 16 * j)]
+            bounds[table[b, j]] = torch.stack((k.amin(0), k.amax(0)), 1)
+    got = ops.paged_kv_bounds(kg, tg, lg, torch.zeros_like(bounds).cuda())
+    assert torch.equal(got.cpu(), bounds)
+    blocks = ops.paged_kv_select(qg, got, tg, lg, 3, block_size=16).cpu()
+    e = ops.paged_kv_evict(mass, tg, lg, 3, block_size=16)
+    m = mass.cpu()
+    for b in (0, 1, 6, 1000, 2047, 4094, 4095):
+        n = -(-int(lens[b]) // 16)
+        at = best(scores(q[b], bounds, [int(p) for p in table[b, :n]])[0].tolist() if n else [], [True] * n, 3, 1, 1)
+        assert blocks[b, 0].tolist() == at + [-1] * (3 - len(at))
+        stay = best(m[b, :n].tolist(), [True] * n, 3, 1, 1)
+        assert e.block_table[b, : len(stay)].tolist() == table[b, stay].tolist() and int(e.evicted_count[b]) == n - len(stay)
+    assert (blocks[:, 0, 0].ge(0) == lens.gt(0)).all() and (e.evicted_count.cpu() == (-(-lens // 16) - 3).clamp(min=0)).all()
+
+
+@pytest.mark.parametrize("block", [65536, 4099])
+def test_the_largest_pages(need_gpu, block):
+    q, kv, table, lens = make(79, [70000, 5, 65537], block, 2, 1, 8, BF16, pages_extra=0, width_extra=0)
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), return_lse=True)
+    check_attention(q, kv, table, lens, out, lse)
+    got = ops.paged_kv_bounds(kv.cuda(), table.cuda(), lens.cuda(), torch.zeros(kv.shape[1], 1, 2, 8, dtype=BF16, device="cuda")).cpu()
+    for b, n in enumerate(lens.tolist()):
+        for j in range(-(-n // block)):
+            k = kv[0, table[b, j], : min(block, n - j * block)]
+            assert torch.equal(got[table[b, j]], torch.stack((k.amin(0), k.amax(0)), 1))
