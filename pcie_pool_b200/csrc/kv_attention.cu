@@ -28,8 +28,8 @@
 //
 // Measured (bf16, 32 heads on 8 key heads of 128, blocks of 16, both kernels, a graph of
 // calls over cold data): 8 x 32768 tokens, 1.07 GB, 163 us, 6.59 TB/s, what a copy
-// reaches; 64 requests of 91 to 8192 tokens, 462 MB, 83 us; 64 x 1024, 268 MB, 52 us;
-// 1 x 16384, 67 MB, 19 us; 1 x 300, 8 us.  What is above the bytes' time is 4 us until
+// reaches; 64 requests of 91 to 8192 tokens, 462 MB, 83 us; 64 x 1024, 268 MB, 53 us;
+// 1 x 16384, 67 MB, 18 us; 1 x 300, 8 us.  What is above the bytes' time is 4 us until
 // the first tiles are asked for (lengths, then pages, each a read from memory), 3 us
 // where a request ends within a range, and 4 us from the last range's end to the
 // join's.  Over a second of such calls the chip is at its power limit and at
@@ -494,7 +494,11 @@ struct Join {
 // tiles for every head (they lie together) over the heads' totals.  The totals of
 // a request that was cut are taken from its parts, eight lanes for a head, since
 // the join beside it only writes them now; the tiles' sums and the old mass are on
-// their way meanwhile.  It adds 2 to 3 us to a call (64 x 1024 tokens: 52 and 55 us).
+// their way meanwhile.  It adds 2 to 3 us to a call (64 x 1024 tokens: 53 and 55 us).
+// A tile's sum waits as its logarithm (base 2, fp32), since the heads' totals are known
+// only at the end: half a step of that is what a weight is off by, as it is by half a step
+// of its score.  CTAs go by the table's width: 256 x 100 tokens take 34 us with 7 columns, 61
+// with 1024, 239 with 8192, where most find nothing to do.
 constexpr int kMassBlocks = kJoinWarps, kMassHeads = 1024, kMassAhead = 8;
 
 __device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, uint32_t cta) {
@@ -557,7 +561,7 @@ __device__ __forceinline__ void add_mass(const KvAttention& a, const Work& w, ui
 // share `units_each` units, 4 * LANES columns of a query head; LANES lanes take a part
 // and a warp 32 / LANES * kJoinParts parts at a time.  With LANES = 8 that is 160 for a
 // CTA: all parts of a request that lies over all SMs are in flight at once.  With a CTA
-// for each request and head, 1024 requests of 16 tokens took 96 us in place of 35.
+// for each request and head, 1024 requests of 16 tokens took 96 us, this way 35 (26 now).
 template <typename T, int LANES, bool MASS>
 __global__ void __launch_bounds__(kJoinWarps * 32, 4)
     attention_join_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ Work w, const __grid_constant__ Join j) {
@@ -709,7 +713,7 @@ cudaError_t launch(const KvAttention& a, const Work& w, int sms, int device, cud
   const uint32_t items = w.by_cut ? w.most_ranges - 1 : a.req.requests;
   // narrow units while the CTAs fit beside the attention's, else whole rows, and
   // as many warps for a unit as leave two CTAs to an SM (1 x 16384 tokens: 20.6 us with
-  // narrow units, 24.2 with rows; 8 x 300: 20.3 with 1024 narrow CTAs, 12.6 this way)
+  // narrow units, 24.2 with rows; 8 x 300: 20.3 with 1024 narrow CTAs, 12.6 this way; 18.1 and 10.2 now)
   auto join = w.z ? attention_join_kernel<T, 8, true> : attention_join_kernel<T, 8, false>;
   auto share_out = [&](int columns, int64_t most) {
     const int units = a.q.heads * ((a.kv.dim + columns - 1) / columns);

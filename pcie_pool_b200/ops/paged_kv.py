@@ -8,7 +8,10 @@ strides that are multiples of 16 bytes with a contiguous last dimension; a
 only: the offloaders take it as it is).  Request ``b`` holds ``context_lens[b]`` tokens, block
 ``j`` of it in page ``block_table[b, j]``.  A table entry that is no page
 (negative, or ``>= pages``) is a block that is not resident -- offloaded, say --
-and its tokens are left out.  Lengths and tables are read on the device when the
+and its tokens are left out.  Where a batch's table is as wide as the longest
+request may get, pass the columns that its requests use (``table[:, :n]``): block
+mass, selection and eviction go by the width (256 requests of 100 tokens with
+mass take 34 us with 7 columns and 239 with 8192).  Lengths and tables are read on the device when the
 kernel runs, so all calls can be captured into a CUDA graph and replayed with
 other contents.
 
@@ -56,7 +59,8 @@ def paged_kv_attention(q, kv, block_table, context_lens, *, scale=None, blocks=N
     ``mass`` fp32 [requests, blocks of the table] is added to in place: the
     attention weight that the heads gave to each block, summed over heads and
     tokens, so a request's row grows by ``heads`` in all.  It needs a block size
-    that is a multiple of 16 and at most 1024 heads, and takes no ``blocks``.
+    that is a multiple of 16 and at most 1024 heads, takes no ``blocks``, and a
+    workspace of ``requests * blocks of the table * block / 16 * heads`` fp32 numbers.
 
     What is not finite in a token that counts shows, and nowhere else: a value that
     is infinite or no number makes that channel of its heads' results infinite or no
