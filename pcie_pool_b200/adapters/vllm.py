@@ -215,7 +215,7 @@ class KVLayout:
 def check_planes(lane_stride: int, block_stride: int, num_blocks: int) -> None:
     """ValueError for a ``[2, num_blocks, ...]`` view whose K and V are not planes of their own: its block
     stride spans both lanes, so a unit would cover its neighbour's keys and the last one end past the cache."""
-    if num_blocks and lane_stride < num_blocks * block_stride:
+    if num_blocks and 0 != lane_stride < num_blocks * block_stride:  # (0: one plane that is both)
         raise ValueError("K and V of a block lie next to each other in this KV tensor: "
                          "pass it as [num_blocks, 2, ...], not as a [2, num_blocks, ...] view")
 

@@ -74,7 +74,8 @@ def test_a_transposed_cache_is_no_cache_of_planes():
 def test_planes_of_any_inner_order_are_taken():
     heads = torch.zeros(2, PAGES, 2, 16, 64, dtype=torch.bfloat16).transpose(2, 3)
     apart = torch.zeros(2, PAGES + 3, 16, 2, 64, dtype=torch.bfloat16)[:, 2: 2 + PAGES]
-    for kv in (heads, apart):
+    both = torch.zeros(1, PAGES, 16, 2, 64, dtype=torch.bfloat16).expand(2, -1, -1, -1, -1)
+    for kv in (heads, apart, both):
         addrs, unit = block_table_units([kv], range(PAGES))
         assert unit == 16 * 2 * 64 * 2 and addrs[-1] == kv.data_ptr() + kv.stride(0) * 2 + (PAGES - 1) * unit
 
