@@ -113,19 +113,20 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-uintptr_t end_of(const Tensor& t) {
+// Bytes that a tensor spans in its dimensions from `dim` on.
+uintptr_t span_of(const Tensor& t, int64_t dim) {
   int64_t last = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-  return address(t) + (last + 1) * t.element_size();
+  for (int64_t i = dim; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return (last + 1) * t.element_size();
 }
 
-// Whether what two tensors span has memory in common.  Rows of one buffer that stand
-// next to each other (equal strides) do not.
+// Whether what two tensors span has memory in common.  Requests' parts of one buffer that
+// stand next to each other (equal strides of the first dimension) do not.
 bool overlaps(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
-  if (address(a) >= end_of(b) || address(b) >= end_of(a)) return false;
-  if (a.dim() != 2 || b.dim() != 2 || a.size(0) < 2 || b.size(0) < 2) return true;
-  const uintptr_t pitch = a.stride(0) * a.element_size(), row_a = a.size(1) * a.element_size(), row_b = b.size(1) * b.element_size();
+  if (address(a) >= address(b) + span_of(b, 0) || address(b) >= address(a) + span_of(a, 0)) return false;
+  if (a.size(0) < 2 || b.size(0) < 2) return true;
+  const uintptr_t pitch = a.stride(0) * a.element_size(), row_a = span_of(a, 1), row_b = span_of(b, 1);
   if (pitch != b.stride(0) * b.element_size() || row_a > pitch || row_b > pitch) return true;
   const uintptr_t apart = address(b) >= address(a) ? (address(b) - address(a)) % pitch : (pitch - (address(a) - address(b)) % pitch) % pitch;
   return apart < row_a || apart + row_b > pitch;

@@ -314,3 +314,19 @@ def test_strides_of_dimensions_of_one_do_not_count():
             ops.paged_kv_attention(q, kv, table, lens)
         with pytest.raises(ValueError, match="multiples of 16 bytes"):
             ops.paged_kv_attention(q, flat.as_strided(sizes, odd), table, lens)
+
+
+def test_what_a_request_has_may_lie_in_one_row(good):
+    """A row a request: its query, its mass and its table next to each other."""
+    n, width = good["block_table"].shape
+    rows = torch.zeros(n, 8 * 64 * 2 + 4 * width + 4 * width + 16, dtype=torch.uint8)
+    q = rows[:, : 8 * 64 * 2].view(torch.bfloat16).unflatten(1, (8, 64)).copy_(good["q"])
+    at = 8 * 64 * 2
+    mass = rows[:, at: at + 4 * width].view(torch.float32)
+    table = rows[:, at + 4 * width: at + 8 * width].view(torch.int32).copy_(good["block_table"])
+    assert not q.is_contiguous() and q.data_ptr() == rows.data_ptr()
+    with pytest.raises(ValueError, match="CUDA device"):
+        ops.paged_kv_attention(**dict(good, q=q, block_table=table), mass=mass)
+    for off in (-4, 4):
+        with pytest.raises(ValueError, match="must not overlap"):
+            ops.paged_kv_attention(**dict(good, q=q, block_table=table), mass=rows[:, at + off: at + off + 4 * width].view(torch.float32))
