@@ -277,7 +277,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> kv_evict(const Tensor
 
 PYBIND11_MODULE(_kv, m) {
   // torch's C++ classes are laid out by version: a module of another one must not run
-  const auto version = py::str(py::module_::import("torch").attr("__version__")).cast<std::string>();
+  // (the installed package's version, which the build took too; torch.__version__ may say more than it)
+  const auto version = py::str(py::module_::import("importlib.metadata").attr("version")("torch")).cast<std::string>();
   if (version != PPB_TORCH)
     throw py::import_error("pcie_pool_b200._kv was built for torch " PPB_TORCH ", this is torch " + version +
                            ": run `python -m pcie_pool_b200._build` and start anew");
