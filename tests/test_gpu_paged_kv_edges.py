@@ -298,3 +298,21 @@ def test_the_largest_pages(need_gpu, block):
         for j in range(-(-n // block)):
             k = kv[0, table[b, j], : min(block, n - j * block)]
             assert torch.equal(got[table[b, j]], torch.stack((k.amin(0), k.amax(0)), 1))
+
+
+# ---- the same block and page again ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("heads", [4, 24])
+def test_the_same_block_and_page_again(need_gpu, heads):
+    """A block listed twice counts twice, a page in two places of a table or in two requests is read in each; of a list only as
+    many entries count as the request has blocks."""
+    q, kv, table, lens = make(80, [75, 75, 33], 16, heads, 2, 64, BF16)
+    table[0, 3] = table[0, 1]
+    table[1] = table[0]
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), return_lse=True)
+    check_attention(q, kv, table, lens, out, lse)
+    blocks = torch.tensor([[[2, 2, 0, 4, 4, 1, 3], [4, 0, 0, 0, 0, 0, 0]], [[1, 3, 1, 3, 0, 2, 2], [0, 1, 2, 3, 4, 0, 1]],
+                           [[2, 2, 2, 0, 1, 0, 1], [1, -1, 1, 2, 2, 2, 2]]], dtype=torch.int32)
+    out, lse = ops.paged_kv_attention(q.cuda(), kv.cuda(), table.cuda(), lens.cuda(), blocks=blocks.cuda(), return_lse=True)
+    check_attention(q, kv, table, lens, out, lse, blocks=blocks)
